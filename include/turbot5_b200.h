@@ -401,6 +401,104 @@ T5B_API int t5b_scatter_rows(const void* packed, int64_t packed_row_stride_bytes
                      int64_t padded_row_stride_bytes, const int32_t* dest, int64_t n_rows,
                      int32_t row_bytes, void* stream);
 
+/* ---- beam search: one step -------------------------------------------------------------
+ * The reference's generation is the one its heads inherit (src/turbot5/heads/t5_heads.py:100-130 prepares its inputs);
+ * no code of its own.  For each of B sentences with num_beams (at most 16) running beams:
+ *
+ *   score[k, t] = scores[k] + logits[k, t] - log(sum_t exp(logits[k, t]))
+ *   candidates: the 2 * num_beams best (k, t); among equal scores the lowest beam, within a beam the largest logit, then
+ *   the lowest token.
+ *
+ * Candidates with t = eos_token_id among the num_beams best join the pool of finished sentences with
+ * score / (pos + 1)^length_penalty; the pool keeps the num_beams best, best first, earlier entries first among equals.
+ * The num_beams best other candidates go on.  The first continuation of a beam takes that beam's place, further ones
+ * the places that are left, in order: a cache then moves for further continuations only.
+ * done: the pool is full and early_stopping, or no running score / (pos + 1)^length_penalty is above the pool's worst;
+ * or every running score is -inf.  A sentence that is done on entry keeps scores and pool, its tokens are pad_token_id,
+ * its parents itself.
+ * NaN logits count as -inf; a row with +inf gives those tokens the whole probability.  Scores are float32, computed and
+ * compared in float64.
+ *   logits (B * num_beams, vocab), row stride in elements, 2 <= vocab <= 2^27; pos: int64 device word, the step's number
+ *   from 0; finished_steps / finished_beams: the step and the parent beam of each finished sentence's end.
+ *   *_out may be the inputs.  history_*: optional int32 (history_steps, B, num_beams), row pos is written. */
+typedef struct {
+  const void* logits; const float* scores; const float* finished_scores; const int32_t* finished_steps;
+  const int32_t* finished_beams; const uint8_t* done; const int64_t* pos;
+  int64_t* tokens_out; int32_t* parents_out; float* scores_out; float* finished_scores_out; int32_t* finished_steps_out;
+  int32_t* finished_beams_out; uint8_t* done_out; int32_t* history_tokens; int32_t* history_parents;
+  int64_t logits_stride, history_steps, eos_token_id, pad_token_id;
+  double length_penalty;
+  int32_t dtype, B, num_beams, vocab, early_stopping;
+} t5b_beam_step_args;
+T5B_API int t5b_beam_search_step(const t5b_beam_step_args* args, void* stream);
+
+/* The num_return best sentences of each search after `steps` steps: the finished ones and, where the search is not done,
+ * the running beams with scores / steps^length_penalty; best first, finished ones first among equals.
+ * tokens / parents int32 (steps, B, num_beams), the step's history; sequences int64 (B, num_return, steps), pad_token_id
+ * behind the end (and throughout where there is no such sentence: score -inf); sequence_scores float32 (B, num_return). */
+typedef struct {
+  const int32_t* tokens; const int32_t* parents; const float* scores; const float* finished_scores;
+  const int32_t* finished_steps; const int32_t* finished_beams; const uint8_t* done;
+  int64_t* sequences; float* sequence_scores;
+  int64_t eos_token_id, pad_token_id;
+  double length_penalty;
+  int32_t steps, B, num_beams, num_return;
+} t5b_beam_sequences_args;
+T5B_API int t5b_beam_search_sequences(const t5b_beam_sequences_args* args, void* stream);
+
+/* ---- beam search: caches follow their beams ------------------------------------------------
+ * In place, for every tensor: row[b * num_beams + j] = row[b * num_beams + parents[b, j]] (all read before any is
+ * written), for the tokens in use.  caches: device pointers to (outer, B * num_beams, H, capacity, token) with byte
+ * strides for the first three dims and token_bytes contiguous bytes per token; scales: float32 (outer, B * num_beams, H,
+ * ceil(capacity / 64)), byte strides, last dim contiguous.  seqlens: optional int32 (B * num_beams), tokens in use (the
+ * longest beam of a sentence counts); NULL: the capacity.  A parent outside the beams leaves its row as it is. */
+#define T5B_CACHE_BLOCK 64
+#define T5B_REORDER_MAX_TENSORS 64
+typedef struct {
+  void* caches[T5B_REORDER_MAX_TENSORS];
+  void* scales[T5B_REORDER_MAX_TENSORS];
+  const int32_t* parents; const int32_t* seqlens;
+  int64_t cache_stride_outer, cache_stride_row, cache_stride_head;
+  int64_t scale_stride_outer, scale_stride_row, scale_stride_head;
+  int32_t n_caches, n_scales, outer, B, num_beams, H, capacity, token_bytes;
+} t5b_cache_reorder_args;
+T5B_API int t5b_beam_cache_reorder(const t5b_cache_reorder_args* args, void* stream);
+
+/* ---- 8-bit caches ------------------------------------------------------------------------------
+ * e4m3 numbers (B, H, capacity, D) with one float32 scale per T5B_CACHE_BLOCK tokens and head, (B, H, capacity / 64):
+ * the smallest power of two s (2^-100 .. 2^120) with max |x| <= 448 s over the block's finite elements.  Infinities
+ * saturate, NaN stays NaN.
+ *
+ * t5b_cache_quantize writes keys and values k, v (B, H, M, D) of `dtype` (element strides, last dim contiguous) at tokens
+ * start .. start + M of the cache; start_ptr: the same from a device word (tokens past the capacity are then dropped).
+ * seqlens: optional int32 (B): only the first seqlens[b] of the M tokens.  Older tokens of a block that is joined move to
+ * its new scale; what lies behind the written tokens is left as it is and counts as empty.  Both caches (and both scale
+ * tensors) have the same strides, in elements; the rows (capacity, D) of a head are contiguous. */
+typedef struct {
+  const void* k; const void* v; void* k_cache; void* v_cache; float* k_scale; float* v_scale;
+  const int64_t* start_ptr; const int32_t* seqlens;
+  int64_t start;
+  int64_t k_stride_b, k_stride_h, k_stride_m, v_stride_b, v_stride_h, v_stride_m;
+  int64_t cache_stride_b, cache_stride_h, scale_stride_b, scale_stride_h;
+  int32_t dtype, B, H, M, D, capacity;
+} t5b_cache_quantize_args;
+T5B_API int t5b_cache_quantize(const t5b_cache_quantize_args* args, void* stream);
+
+/* t5b_decode_fwd against such a cache: q, out (B, H, M, D) fp16 or bf16; the first N (seqlens_k[b]) tokens of k and v;
+ * q_pos_offset < 0: the key length - M.  A row that sees no key gives zeros.  No workspace. */
+typedef struct {
+  const void* q; const void* k; const void* v; const float* k_scale; const float* v_scale; void* out;
+  const void* table; const int32_t* seqlens_k;
+  int64_t q_stride_b, q_stride_h, q_stride_m;
+  int64_t k_stride_b, k_stride_h, v_stride_b, v_stride_h;
+  int64_t k_scale_stride_b, k_scale_stride_h, v_scale_stride_b, v_scale_stride_h;
+  int64_t o_stride_b, o_stride_h, o_stride_m;
+  int64_t table_stride0;
+  int32_t dtype, table_dtype, B, H, M, N, D, causal, num_buckets, max_distance, q_pos_offset;
+  float sm_scale;
+} t5b_decode_quantized_args;
+T5B_API int t5b_decode_quantized_fwd(const t5b_decode_quantized_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

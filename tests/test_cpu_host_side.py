@@ -276,3 +276,81 @@ def test_forward_kernels_of_every_form_of_call_stay_within_their_budget():
     assert len(forms) == 2 * 2 * 4          # types, head dims, forms
     for n, k in forms.items():
         assert k["registers"] <= 96 and k["spill_stores"] <= 24, (n, k)
+
+
+def _c_struct(cname):
+    """The ctypes form of a struct in the header, arrays included."""
+    header = open(os.path.join(ROOT, "include", "turbot5_b200.h")).read()
+    end = header.index("} " + cname + ";")
+    body = re.sub(r"/\*.*?\*/", "", header[header.rindex("typedef struct {", 0, end) + len("typedef struct {"):end], flags=re.S)
+    consts = {k: int(v) for k, v in re.findall(r"#define (T5B_\w+) (\d+)", header)}
+    types = {"int64_t": ctypes.c_int64, "int32_t": ctypes.c_int32, "float": ctypes.c_float, "double": ctypes.c_double}
+    fields = []
+    for decl in filter(None, (d.strip() for d in body.split(";"))):
+        base = ctypes.c_void_p if "*" in decl else types[decl.split()[0]]
+        names = decl.replace("*", " ").split(",")
+        for name in [names[0].split()[-1]] + [n.strip() for n in names[1:]]:
+            m = re.match(r"(\w+)\[(\w+)\]", name)
+            fields.append((m.group(1), base * consts[m.group(2)]) if m else (name, base))
+    return type(cname, (ctypes.Structure,), {"_fields_": fields})
+
+
+def test_generation_entry_points_validate_arguments_without_a_device():
+    from turbot5_b200 import _native as nat
+    L = nat.lib()
+    ptr = lambda a: ctypes.cast(ctypes.byref(a), ctypes.c_void_p)
+    for name in ("t5b_beam_search_step", "t5b_beam_search_sequences", "t5b_beam_cache_reorder", "t5b_cache_quantize", "t5b_decode_quantized_fwd"):
+        assert getattr(L, name)(None, None) == 5, name
+    Step = _c_struct("t5b_beam_step_args")
+    good = dict(dtype=nat.BF16, B=1, num_beams=4, vocab=100)
+    for change, status in ((dict(dtype=9), 1), (dict(num_beams=17), 2), (dict(num_beams=0), 2), (dict(vocab=1), 2), (dict(vocab=(1 << 27) + 1), 2),
+                           (dict(B=-1), 2), (dict(B=0), 0), ({}, 5)):
+        assert L.t5b_beam_search_step(ptr(Step(**{**good, **change})), None) == status, change
+    full = {n: 16 for n in ("logits", "scores", "finished_scores", "finished_steps", "finished_beams", "done", "pos", "tokens_out", "parents_out",
+                            "scores_out", "finished_scores_out", "finished_steps_out", "finished_beams_out", "done_out")}
+    for change, status in ((dict(logits=17), 3), (dict(history_tokens=16), 5), (dict(length_penalty=float("nan")), 5)):
+        assert L.t5b_beam_search_step(ptr(Step(**{**good, **full, **change})), None) == status, change
+    Seq = _c_struct("t5b_beam_sequences_args")
+    good = dict(steps=3, B=1, num_beams=4, num_return=1)
+    for change, status in ((dict(steps=0), 2), (dict(num_return=5), 2), (dict(num_return=0), 2), (dict(num_beams=20), 2), (dict(B=0), 0), ({}, 5)):
+        assert L.t5b_beam_search_sequences(ptr(Seq(**{**good, **change})), None) == status, change
+    Re = _c_struct("t5b_cache_reorder_args")
+    good = dict(n_caches=1, outer=2, B=1, num_beams=4, H=2, capacity=8, token_bytes=128, parents=16)
+    for change, status in ((dict(n_caches=65), 2), (dict(token_bytes=0), 2), (dict(num_beams=17), 2), (dict(n_caches=0), 0), (dict(capacity=0), 0),
+                           (dict(parents=None), 5), ({}, 5), (dict(capacity=1 << 30), 5)):
+        assert L.t5b_beam_cache_reorder(ptr(Re(**{**good, **change})), None) == status, change
+    Fill = _c_struct("t5b_cache_quantize_args")
+    good = dict(dtype=nat.F16, B=1, H=2, M=4, D=64, capacity=64)
+    for change, status in ((dict(dtype=5), 1), (dict(D=48), 4), (dict(capacity=60), 2), (dict(M=-1), 2), (dict(start=-1), 5), (dict(M=0), 0), ({}, 5)):
+        assert L.t5b_cache_quantize(ptr(Fill(**{**good, **change})), None) == status, change
+    full = {n: 16 for n in ("k", "v", "k_cache", "v_cache", "k_scale", "v_scale")}
+    for change, status in ((dict(start=61), 2), (dict(k=17), 3), (dict(k_cache=24), 3), (dict(cache_stride_h=8), 3)):
+        assert L.t5b_cache_quantize(ptr(Fill(**{**good, **full, **change})), None) == status, change
+    Att = _c_struct("t5b_decode_quantized_args")
+    good = dict(dtype=nat.BF16, B=1, H=2, M=1, N=64, D=64)
+    for change, status in ((dict(dtype=nat.F32), 1), (dict(D=20), 4), (dict(N=-1), 2), (dict(H=70000), 2), (dict(M=0), 0), ({}, 5)):
+        assert L.t5b_decode_quantized_fwd(ptr(Att(**{**good, **change})), None) == status, change
+    full = {n: 16 for n in ("q", "k", "v", "k_scale", "v_scale", "out")}
+    for change, status in ((dict(k=24), 3), (dict(v_stride_h=8), 3), (dict(table=16, table_dtype=7), 1),
+                           (dict(table=16, num_buckets=2, max_distance=128), 5)):
+        assert L.t5b_decode_quantized_fwd(ptr(Att(**{**good, **full, **change})), None) == status, change
+
+
+def test_generation_operators_refuse_cpu_tensors():
+    import turbot5_b200 as t5b
+    s, i = torch.zeros((2, 4)), torch.zeros((2, 4), dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        t5b.beam_search_step(torch.zeros((8, 50)), s, s, i, i, torch.zeros(2, dtype=torch.bool), torch.zeros(1, dtype=torch.long))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        t5b.beam_search_sequences(i[None], i[None], s, s, i, i, torch.zeros(2, dtype=torch.bool))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        t5b.reorder_beam_cache([torch.zeros((8, 1, 2, 4))], i)
+    x, c, sc = torch.zeros((1, 1, 2, 16), dtype=torch.bfloat16), torch.zeros((1, 1, 64, 16)).to(torch.float8_e4m3fn), torch.zeros((1, 1, 1))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        t5b.quantize_into_cache(x, x, c, sc, c, sc)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        t5b.flash_decoding_quantized_with_fusing_bias(x, c, sc, c, sc, None)
+    with pytest.raises(TypeError):
+        t5b.reorder_beam_cache(3, i)
+    with pytest.raises(TypeError):
+        t5b.beam_search_step(None, s, s, i, i, None, None)

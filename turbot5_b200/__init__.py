@@ -7,9 +7,10 @@ other backend: operators raise if the library is missing or a tensor is not on a
 CUDA device.
 """
 from .attention import (check_device_status, flash_attention_partial, flash_attention_with_fusing_bias,
-                        flash_attention_with_fusing_bias_varlen, flash_decoding_with_fusing_bias,
-                        merge_attention_partials, relative_position_bucket_grid, relative_position_bucket_table)
-
+                        flash_attention_with_fusing_bias_varlen, flash_decoding_quantized_with_fusing_bias,
+                        flash_decoding_with_fusing_bias, merge_attention_partials, relative_position_bucket_grid,
+                        relative_position_bucket_table)
+from .generation import beam_search_sequences, beam_search_step, quantize_into_cache, reorder_beam_cache
 from .modules import (RMSLayerNorm, T5ATTENTION_TYPES, T5FlashAttention, T5LayerNorm, T5LocalFlashAttention,
                       add_rms_layer_norm, gated_gelu, rms_layer_norm)
 from .padding import get_unpad_plan, pad_rows, unpad_rows
@@ -22,6 +23,8 @@ __all__ = [
     "add_rms_layer_norm", "gated_gelu", "flash_attention_partial", "merge_attention_partials",
     "sequence_parallel_attention", "sequence_parallel_attention_overlapped", "shard_bounds", "shard_size",
     "flash_attention_with_fusing_bias", "flash_attention_with_fusing_bias_varlen",
-    "flash_decoding_with_fusing_bias", "relative_position_bucket_table",
+    "flash_decoding_with_fusing_bias", "flash_decoding_quantized_with_fusing_bias",
+    "beam_search_step", "beam_search_sequences", "reorder_beam_cache", "quantize_into_cache",
+    "relative_position_bucket_table",
     "relative_position_bucket_grid", "check_device_status",
 ]

@@ -29,7 +29,9 @@ SYMBOLS = ("t5b_status_string", "t5b_abi_version", "t5b_bucket_table_host", "t5b
            "t5b_decoder_step_workspace_bytes", "t5b_decoder_step_prepare", "t5b_decoder_step",
            "t5b_rmsnorm_fwd", "t5b_rmsnorm_bwd", "t5b_rmsnorm_bwd_add", "t5b_gated_gelu_bwd", "t5b_unpad_plan", "t5b_gather_rows",
            "t5b_scatter_rows", "t5b_attention_merge", "t5b_add_rmsnorm_fwd", "t5b_gated_gelu_fwd",
-           "t5b_check_status", "t5b_selftest_bounded_wait", "t5b_selftest_decoder_wait")
+           "t5b_check_status", "t5b_selftest_bounded_wait", "t5b_selftest_decoder_wait",
+           "t5b_beam_search_step", "t5b_beam_search_sequences", "t5b_beam_cache_reorder", "t5b_cache_quantize",
+           "t5b_decode_quantized_fwd")
 
 
 class AttnArgs(C.Structure):
@@ -158,6 +160,11 @@ def lib():
     L.t5b_gated_gelu_fwd.restype = C.c_int
     L.t5b_gated_gelu_fwd.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int64, C.c_int64, C.c_int32,
                                      C.c_void_p]
+    for name in ("t5b_beam_search_step", "t5b_beam_search_sequences", "t5b_beam_cache_reorder", "t5b_cache_quantize",
+                 "t5b_decode_quantized_fwd"):
+        fn = getattr(L, name)
+        fn.restype = C.c_int
+        fn.argtypes = [C.c_void_p, C.c_void_p]
     for name in ("t5b_gather_rows", "t5b_scatter_rows"):
         fn = getattr(L, name)
         fn.restype = C.c_int

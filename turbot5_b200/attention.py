@@ -132,6 +132,20 @@ def flash_decoding_with_fusing_bias(q, k, v, bias, causal=False, sm_scale=None, 
                         num_splits, workspace)
 
 
+def flash_decoding_quantized_with_fusing_bias(q, k, k_scale, v, v_scale, bias, causal=False, sm_scale=None, NUM_BUCKETS=32,
+                                              MAX_DISTANCE=128, *, kv_len=None, seqlens_k=None, q_pos_offset=None):
+    """`flash_decoding_with_fusing_bias` against an 8-bit cache: q (B,H,M,D) in float16 or bfloat16 with small M, keys and
+    values (B,H,cap,D) in float8_e4m3fn with one float32 scale per 64 tokens and head (B,H,cap/64), as
+    `quantize_into_cache` leaves them.
+
+    Half of the bytes of a 16-bit cache are read; up to eight query rows (the beams of a sentence against its encoder's
+    keys) cost one pass over them.  Only the first `kv_len` (`seqlens_k[b]`) keys are read; a row that sees none gives
+    zeros.  A key that is visible to some rows of a causal call only must hold finite numbers: 0 x NaN is NaN.  No
+    workspace and no state: calls on any streams are independent.  No gradients are recorded."""
+    return _host.decode_quantized(q, k, k_scale, v, v_scale, bias, causal, sm_scale, NUM_BUCKETS, MAX_DISTANCE, kv_len,
+                                  seqlens_k, q_pos_offset)
+
+
 def relative_position_bucket_table(num_buckets=32, max_distance=128, bidirectional=True,
                                    lo=None, hi=None) -> torch.Tensor:
     """bucket(delta) for delta in [lo, hi] as an int32 CPU tensor (host table of the library)."""

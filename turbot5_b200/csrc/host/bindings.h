@@ -48,5 +48,6 @@ inline void expect(Py_ssize_t got, Py_ssize_t want) { TORCH_CHECK_TYPE(got == wa
 
 #define T5B_METHOD(name, fn) {name, (PyCFunction)(void (*)(void))fn, METH_FASTCALL, nullptr}
 extern PyMethodDef stack_methods[];
+extern PyMethodDef generation_methods[];
 
 }  // namespace t5b_host

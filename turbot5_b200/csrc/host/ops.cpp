@@ -787,6 +787,9 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "Native host side of the 
 
 PyMODINIT_FUNC PyInit__host(void) {
   PyObject* m = PyModule_Create(&t5b_host::kModule);
-  if (m && PyModule_AddFunctions(m, t5b_host::stack_methods) < 0) { Py_DECREF(m); return nullptr; }
+  if (m && (PyModule_AddFunctions(m, t5b_host::stack_methods) < 0 || PyModule_AddFunctions(m, t5b_host::generation_methods) < 0)) {
+    Py_DECREF(m);
+    return nullptr;
+  }
   return m;
 }

@@ -1,0 +1,319 @@
+// Decoder caches: keys and values into 8-bit blocks, and the reordering of beams.
+//
+// An 8-bit cache holds e4m3 numbers (B, H, capacity, D) and one float32 scale per 64 tokens and head, a power of two:
+//
+//   scale = the smallest 2^e with max |x| <= 448 * 2^e  (-100 <= e <= 120),   stored = round_e4m3(x / scale)
+//
+// With a power of two the division is exact, so one rounding of three mantissa bits is all that is lost, and tokens that
+// join a block with a larger scale move the older ones by whole exponents: nothing is rounded twice unless it falls
+// below the smallest normal number of the format.
+//
+// The reference keeps its cache in the model's type and reorders it with index_select per tensor
+// (src/turbot5/model/attentions.py:198,229-234; src/turbot5/heads/t5_heads.py:100-130 inherits the generation loop).
+#include "t5b_common.cuh"
+
+namespace t5b {
+namespace kvcache {
+
+constexpr int BLOCK = T5B_CACHE_BLOCK;
+constexpr int LOWEST = -100, HIGHEST = 120;
+
+// two floats -> two e4m3 numbers, nearest even, saturating (NaN stays NaN)
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// exponent of the scale for a block whose largest finite magnitude has these bits
+__device__ __forceinline__ int scale_exponent(uint32_t bits) {
+  // |x| = 1.f * 2^e; 448 = 1.75 * 2^8: one more where 1.f > 1.75 (below the normal numbers the clamp decides)
+  const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return min(max(e, LOWEST), HIGHEST);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+struct FillParams {
+  const void* src[2]; uint8_t* cache[2]; float* scale[2];
+  int64_t src_b[2], src_h[2], src_m[2];       // element strides
+  int64_t cache_b[2], cache_h[2], scale_b[2], scale_h[2];
+  const int64_t* start_ptr; int64_t start;
+  const int32_t* seqlens;
+  int32_t B, H, M, cap;
+  int32_t aligned[2];                         // 8 elements of a row start on 16 bytes
+};
+
+// eight consecutive elements of a row
+template <typename T> __device__ __forceinline__ void load8(const T* p, bool aligned, float (&x)[8]) {
+  if (aligned) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = __ldg((const float4*)p), b = __ldg((const float4*)p + 1);
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+      const uint4 u = __ldg((const uint4*)p);
+      const T* t = reinterpret_cast<const T*>(&u);
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = to_float<T>(t[i]);
+    }
+  } else {
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float<T>(p[i]);
+  }
+}
+__device__ __forceinline__ uint32_t magnitude(float x) {
+  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;            // infinities saturate, NaN stays NaN: neither sets a scale
+}
+__device__ __forceinline__ uint2 pack8(const float (&x)[8], float inv) {
+  return make_uint2(to_e4m3x2(x[0] * inv, x[1] * inv) | to_e4m3x2(x[2] * inv, x[3] * inv) << 16,
+                    to_e4m3x2(x[4] * inv, x[5] * inv) | to_e4m3x2(x[6] * inv, x[7] * inv) << 16);
+}
+__device__ __forceinline__ uint2 rescale8(uint2 v, float f) {
+  const float2 a = from_e4m3x2(v.x & 0xffffu), b = from_e4m3x2(v.x >> 16), c = from_e4m3x2(v.y & 0xffffu), d = from_e4m3x2(v.y >> 16);
+  const float x[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+  return pack8(x, f);
+}
+
+// A team of TEAM threads fills one block of 64 tokens of one head, keys or values.  TEAM 128 for prompts: every thread
+// holds its share of the block in registers between the search for the largest and the rounding (one read of the
+// source).  TEAM 32 for single tokens: a warp has one row to write, four heads share a block of threads.
+template <typename T, int D, int TEAM>
+__global__ void __launch_bounds__(128)
+fill_kernel(const __grid_constant__ FillParams p) {
+  constexpr int PARTS = D / 8;                                     // 8-element pieces of a row
+  constexpr int PER = TEAM == 32 ? 1 : BLOCK * PARTS / TEAM;       // pieces per thread
+  __shared__ uint32_t largest[4];
+  const int lane = threadIdx.x % TEAM;
+  const int head = TEAM == 32 ? blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
+  const int b = blockIdx.z >> 1, kv = blockIdx.z & 1;
+  if (TEAM == 32 && head >= p.H) return;                           // whole warps
+  const int64_t start = p.start_ptr ? *p.start_ptr : p.start;
+  const int count = p.seqlens ? min(max(p.seqlens[b], 0), p.M) : p.M;
+  const int64_t end = min(start + (int64_t)count, (int64_t)p.cap);
+  const int64_t first = (start / BLOCK + blockIdx.y) * BLOCK;      // the block's first token
+  const int64_t lo = first > start ? first : start, hi = first + BLOCK < end ? first + BLOCK : end;
+  if (start < 0 || lo >= hi) return;                               // the same for the whole team
+  const T* src = (const T*)p.src[kv] + (int64_t)b * p.src_b[kv] + (int64_t)head * p.src_h[kv];
+  uint8_t* cache = p.cache[kv] + (int64_t)b * p.cache_b[kv] + (int64_t)head * p.cache_h[kv];
+  float* scale = p.scale[kv] + (int64_t)b * p.scale_b[kv] + (int64_t)head * p.scale_h[kv] + first / BLOCK;
+
+  float x[PER][8];
+  uint32_t most = 0;
+  #pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int piece = lane + i * TEAM;
+    const int64_t token = (TEAM == 32 ? lo : first) + piece / PARTS;
+    const bool in = TEAM == 32 ? piece < PARTS : token >= lo && token < hi;
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
+    if (in) load8<T>(src + (token - start) * p.src_m[kv] + piece % PARTS * 8, p.aligned[kv], x[i]);
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) most = max(most, magnitude(x[i][j]));
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (TEAM > 32) {
+    if ((threadIdx.x & 31) == 0) largest[threadIdx.x / 32] = most;
+    __syncthreads();
+    most = max(max(largest[0], largest[1]), max(largest[2], largest[3]));
+  }
+  float now = pow2(scale_exponent(most));
+  const bool kept = lo > first;                                    // older tokens share the block
+  const float was = kept ? *scale : 0.f;
+  now = fmaxf(now, was);
+  const float inv = 1.f / now;
+  if (kept && now > was) {
+    // the older tokens follow to the larger scale
+    const float f = was * inv;
+    for (int i = lane; i < (int)(lo - first) * PARTS; i += TEAM) {
+      uint2* at = (uint2*)(cache + first * D) + i;
+      *at = rescale8(*at, f);
+    }
+  }
+  #pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int piece = lane + i * TEAM;
+    const int64_t token = (TEAM == 32 ? lo : first) + piece / PARTS;
+    const bool in = TEAM == 32 ? piece < PARTS : token >= lo && token < hi;
+    if (in) *(uint2*)(cache + token * D + piece % PARTS * 8) = pack8(x[i], inv);
+  }
+  if (TEAM == 32) __syncwarp(); else __syncthreads();              // every thread has read the old scale
+  if (lane == 0) *scale = now;
+}
+
+// ---- reordering of beams -------------------------------------------------------------------------------------------
+//
+// Bound by the bytes of the beams that change.  A thread owns one offset of all beams of a sentence: it loads what the
+// changed beams are to become, then stores it, so the caches are permuted in place without a second copy and without
+// ordering between threads, whatever the parents are.  Beams that stay are neither read nor written, nor is what lies
+// behind the tokens in use; all layers are one launch.
+constexpr int REORDER_THREADS = 256;
+
+struct ReorderGroup {
+  void* base[T5B_REORDER_MAX_TENSORS];
+  int64_t outer_b, row_b, head_b;       // byte strides of dims 0, 1, 2
+  int32_t n, outer, unit_per_block;     // tensors; dim 0; units per token block (see below)
+  int32_t tokens_per_unit_block;        // 1 for caches (a token), 64 for scales
+};
+struct ReorderParams {
+  ReorderGroup g[2];
+  const int32_t* parents; const int32_t* seqlens;
+  int32_t K, H, cap;
+};
+
+template <typename U, int KM>
+__device__ __forceinline__ void reorder_group(const ReorderParams& p, const ReorderGroup& g, int z, int b, int len,
+                                              const int (&parent)[KM], uint32_t changed) {
+  char* base = (char*)g.base[z / g.outer] + (int64_t)(z % g.outer) * g.outer_b + (int64_t)b * p.K * g.row_b;
+  const int per_head = (len + g.tokens_per_unit_block - 1) / g.tokens_per_unit_block * g.unit_per_block;
+  const int total = per_head * p.H;
+  for (int i = blockIdx.x * REORDER_THREADS + threadIdx.x; i < total; i += gridDim.x * REORDER_THREADS) {
+    const int h = i / per_head;
+    U* at = (U*)(base + (int64_t)h * g.head_b) + (i - h * per_head);
+    U v[KM];
+    #pragma unroll
+    for (int j = 0; j < KM; ++j)
+      if (changed >> j & 1) v[j] = *(U*)((char*)at + (int64_t)parent[j] * g.row_b);
+    #pragma unroll
+    for (int j = 0; j < KM; ++j)
+      if (changed >> j & 1) *(U*)((char*)at + (int64_t)j * g.row_b) = v[j];
+  }
+}
+
+template <typename U, int KM>
+__global__ void __launch_bounds__(REORDER_THREADS)
+reorder_kernel(const __grid_constant__ ReorderParams p) {
+  const int b = blockIdx.z, K = p.K;
+  int parent[KM], len = 0;
+  uint32_t changed = 0;
+  #pragma unroll
+  for (int j = 0; j < KM; ++j) {
+    parent[j] = j;
+    if (j < K) {
+      const int q = p.parents[(int64_t)b * K + j];
+      if (q >= 0 && q < K && q != j) { parent[j] = q; changed |= 1u << j; }
+      if (p.seqlens) len = max(len, p.seqlens[(int64_t)b * K + j]);
+    }
+  }
+  if (!changed) return;
+  len = p.seqlens ? min(len, p.cap) : p.cap;
+  const int caches = p.g[0].n * p.g[0].outer, z = blockIdx.y;
+  if (z < caches) reorder_group<U, KM>(p, p.g[0], z, b, len, parent, changed);
+  else reorder_group<uint32_t, KM>(p, p.g[1], z - caches, b, len, parent, changed);
+}
+
+template <typename U>
+static int launch_reorder(const ReorderParams& p, int B, int64_t units, cudaStream_t stream) {
+  const int tensors = p.g[0].n * p.g[0].outer + p.g[1].n * p.g[1].outer;
+  // four offsets per thread at the cache's capacity; what lies behind the tokens in use ends at once
+  const int64_t blocks = (units + 4 * REORDER_THREADS - 1) / (4 * REORDER_THREADS);
+  const dim3 grid((unsigned)(blocks < 1 ? 1 : blocks > 1024 ? 1024 : blocks), (unsigned)tensors, (unsigned)B);
+  if (p.K <= 4) reorder_kernel<U, 4><<<grid, REORDER_THREADS, 0, stream>>>(p);
+  else if (p.K <= 8) reorder_kernel<U, 8><<<grid, REORDER_THREADS, 0, stream>>>(p);
+  else reorder_kernel<U, 16><<<grid, REORDER_THREADS, 0, stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? T5B_OK : T5B_ERR_LAUNCH;
+}
+
+template <typename T, int D>
+static int launch_fill(const FillParams& p, cudaStream_t stream) {
+  if (p.M == 1) {
+    fill_kernel<T, D, 32><<<dim3((p.H + 3) / 4, 1, 2 * p.B), 128, 0, stream>>>(p);
+  } else {
+    const int blocks = (p.M + BLOCK - 2) / BLOCK + 1;      // wherever the first token stands in its block
+    fill_kernel<T, D, 128><<<dim3(p.H, blocks, 2 * p.B), 128, 0, stream>>>(p);
+  }
+  return cudaGetLastError() == cudaSuccess ? T5B_OK : T5B_ERR_LAUNCH;
+}
+
+template <typename T>
+static int launch_fill_d(const FillParams& p, int D, cudaStream_t stream) {
+  switch (D) {
+    case 16: return launch_fill<T, 16>(p, stream);
+    case 32: return launch_fill<T, 32>(p, stream);
+    case 64: return launch_fill<T, 64>(p, stream);
+    case 128: return launch_fill<T, 128>(p, stream);
+  }
+  return T5B_ERR_HEAD_DIM;
+}
+
+}  // namespace kvcache
+}  // namespace t5b
+
+using namespace t5b;
+
+extern "C" int t5b_cache_quantize(const t5b_cache_quantize_args* a, void* stream) {
+  if (!a) return T5B_ERR_ARG;
+  if (a->dtype != T5B_F32 && a->dtype != T5B_F16 && a->dtype != T5B_BF16) return T5B_ERR_DTYPE;
+  if (a->D != 16 && a->D != 32 && a->D != 64 && a->D != 128) return T5B_ERR_HEAD_DIM;
+  if (a->B < 0 || a->H < 0 || a->M < 0 || a->capacity < 0 || a->capacity % T5B_CACHE_BLOCK || a->B > 32767 || a->H > 65535 ||
+      (a->M + T5B_CACHE_BLOCK - 2) / T5B_CACHE_BLOCK + 1 > 65535) return T5B_ERR_SHAPE;
+  if (!a->start_ptr && a->start < 0) return T5B_ERR_ARG;
+  if (a->B == 0 || a->H == 0 || a->M == 0) return T5B_OK;
+  if (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale) return T5B_ERR_ARG;
+  if (!a->start_ptr && a->start + a->M > a->capacity) return T5B_ERR_SHAPE;
+  const int es = dtype_bytes(a->dtype);
+  kvcache::FillParams p;
+  p.src[0] = a->k; p.src[1] = a->v;
+  p.cache[0] = (uint8_t*)a->k_cache; p.cache[1] = (uint8_t*)a->v_cache;
+  p.scale[0] = a->k_scale; p.scale[1] = a->v_scale;
+  p.src_b[0] = a->k_stride_b; p.src_h[0] = a->k_stride_h; p.src_m[0] = a->k_stride_m;
+  p.src_b[1] = a->v_stride_b; p.src_h[1] = a->v_stride_h; p.src_m[1] = a->v_stride_m;
+  for (int i = 0; i < 2; ++i) {
+    p.cache_b[i] = a->cache_stride_b; p.cache_h[i] = a->cache_stride_h;
+    p.scale_b[i] = a->scale_stride_b; p.scale_h[i] = a->scale_stride_h;
+    if ((uintptr_t)p.src[i] % es) return T5B_ERR_ALIGN;
+    p.aligned[i] = (uintptr_t)p.src[i] % 16 == 0 && p.src_b[i] * es % 16 == 0 && p.src_h[i] * es % 16 == 0 && p.src_m[i] * es % 16 == 0;
+    if ((uintptr_t)p.cache[i] % 16 || (uintptr_t)p.scale[i] % 4) return T5B_ERR_ALIGN;
+  }
+  if (a->cache_stride_b % 16 || a->cache_stride_h % 16) return T5B_ERR_ALIGN;
+  p.start_ptr = a->start_ptr; p.start = a->start; p.seqlens = a->seqlens;
+  p.B = a->B; p.H = a->H; p.M = a->M; p.cap = a->capacity;
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (a->dtype) {
+    case T5B_F32: return kvcache::launch_fill_d<float>(p, a->D, st);
+    case T5B_F16: return kvcache::launch_fill_d<__half>(p, a->D, st);
+    default: return kvcache::launch_fill_d<__nv_bfloat16>(p, a->D, st);
+  }
+}
+
+extern "C" int t5b_beam_cache_reorder(const t5b_cache_reorder_args* a, void* stream) {
+  if (!a) return T5B_ERR_ARG;
+  if (a->B < 0 || a->num_beams < 1 || a->num_beams > 16 || a->H < 0 || a->capacity < 0 || a->outer < 0 || a->n_caches < 0 ||
+      a->n_scales < 0 || a->token_bytes < 1 || a->n_caches > T5B_REORDER_MAX_TENSORS || a->n_scales > T5B_REORDER_MAX_TENSORS ||
+      a->B > 65535 || (int64_t)(a->n_caches + a->n_scales) * a->outer > 65535) return T5B_ERR_SHAPE;
+  if (a->B == 0 || a->H == 0 || a->capacity == 0 || a->outer == 0 || a->n_caches + a->n_scales == 0) return T5B_OK;
+  if (!a->parents) return T5B_ERR_ARG;
+  kvcache::ReorderParams p;
+  kvcache::ReorderGroup& c = p.g[0];
+  kvcache::ReorderGroup& s = p.g[1];
+  uint64_t all = (uint64_t)(a->cache_stride_outer | a->cache_stride_row | a->cache_stride_head | a->token_bytes);
+  for (int i = 0; i < a->n_caches; ++i) {
+    if (!a->caches[i]) return T5B_ERR_ARG;
+    c.base[i] = a->caches[i];
+    all |= (uint64_t)(uintptr_t)a->caches[i];
+  }
+  uint64_t sall = (uint64_t)(a->scale_stride_outer | a->scale_stride_row | a->scale_stride_head);
+  for (int i = 0; i < a->n_scales; ++i) {
+    if (!a->scales[i]) return T5B_ERR_ARG;
+    s.base[i] = a->scales[i];
+    sall |= (uint64_t)(uintptr_t)a->scales[i];
+  }
+  if (a->n_scales && sall % 4) return T5B_ERR_ALIGN;
+  const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;     // whole units on every way through the strides
+  c.outer_b = a->cache_stride_outer; c.row_b = a->cache_stride_row; c.head_b = a->cache_stride_head;
+  c.n = a->n_caches; c.outer = a->outer; c.unit_per_block = a->token_bytes / unit; c.tokens_per_unit_block = 1;
+  s.outer_b = a->scale_stride_outer; s.row_b = a->scale_stride_row; s.head_b = a->scale_stride_head;
+  s.n = a->n_scales; s.outer = a->outer; s.unit_per_block = 1; s.tokens_per_unit_block = T5B_CACHE_BLOCK;
+  p.parents = a->parents; p.seqlens = a->seqlens;
+  p.K = a->num_beams; p.H = a->H; p.cap = a->capacity;
+  const int64_t units = (int64_t)a->capacity * c.unit_per_block * a->H;
+  if (units > 0x7fffffffll - 1024ll * kvcache::REORDER_THREADS) return T5B_ERR_SHAPE;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (unit == 16) return kvcache::launch_reorder<uint4>(p, a->B, units, st);
+  if (unit == 4) return kvcache::launch_reorder<uint32_t>(p, a->B, units, st);
+  return kvcache::launch_reorder<uint8_t>(p, a->B, units, st);
+}
