@@ -7,19 +7,28 @@
 //   the 2K best (k, t): by s, then the lowest beam, then the largest logit, then the lowest token
 //   -> those that end the sentence join the pool of finished sentences, the K best others go on.
 //
-// One cluster of blocks per sentence reads every logit once.  A warp owns a slice of one beam's row (a "unit") and
-// keeps the slice's maximum and sum of exponentials; after one exchange over the cluster's shared memory every block
-// knows lse[] and the maxima of all slices.  The n-th largest of those maxima (as scores) is a bound that n
-// candidates reach, so only lanes whose own maximum reaches it look at their elements again: for n = 8 out of 128
-// slices about nine candidates are left, and one block ranks them by counting.  Where the bound does not thin the
-// candidates out (fewer finite ones than n, or hundreds of equal ones) every warp makes the sorted list of its slice's
-// n best instead and one block merges the lists.  Sums of exponentials are float32 within a lane (a few dozen terms)
-// and float64 from there on, as are the scores: two candidates of different beams are told apart to about 1e-8.
+// One cluster of blocks per sentence reads every logit once; a warp owns a slice of one running beam's row (a "unit").
+// What a kernel of this size costs is not the bytes but the steps that wait for one another (a cluster barrier is some 900
+// cycles, more than the pass over a block's 32 KB), so there is one exchange:
+//
+//   * In a block, the warps of one row form a segment.  The n-th largest of the maxima of 33 to 64 groups of its lanes is
+//     a bound that n of its elements reach, so only lanes whose own maximum reaches it look at their elements again: for
+//     n = 8 about nine candidates per segment are left.
+//   * Those and the slices' maxima and sums of exponentials go to the cluster's first block, which makes the log-sums,
+//     scores the candidates, thins them out by the same bound where they are many (n = 32) and ranks the rest by counting.
+//   * Where that fails - fewer finite candidates than n, or hundreds of equal ones - every warp makes the sorted list of its
+//     slice's n best instead and the first block merges the lists.
+//
+// Sums of exponentials are float32 within a lane (a few dozen terms) and float64 from there on, as are the scores: two
+// candidates of different beams are told apart to about 1e-8.
 //
 // The reference has no beam search of its own (its heads inherit it: src/turbot5/heads/t5_heads.py:100-130).
 #include "t5b_common.cuh"
 
 #include <cooperative_groups.h>
+
+#include <atomic>
+#include <type_traits>
 
 namespace cg = cooperative_groups;
 
@@ -28,12 +37,11 @@ namespace beam {
 
 constexpr int WARPS = 16;
 constexpr int THREADS = WARPS * 32;
-constexpr int MAX_CLUSTER = 8;
+constexpr int MAX_CLUSTER = 16;          // more than 8 is beyond what every GPU has to offer, but not this one
 constexpr int MAX_UNITS = WARPS * MAX_CLUSTER;
-constexpr int MAX_GROUPS = 128;          // maxima that the bound is taken from
-constexpr int MAX_SURVIVORS = 256;
+constexpr int MAX_FOUND = 1024;          // candidates of a sentence, an equal share for each block of the cluster
+constexpr int FEW = 128;                 // candidates that are ranked by counting without another bound
 constexpr int MAX_BEAMS = 16;
-constexpr int MAX_CAND = 2 * MAX_BEAMS;  // one candidate per lane in the end
 constexpr int TOKEN_BITS = 27;
 constexpr uint32_t TOKEN_MASK = (1u << TOKEN_BITS) - 1;
 
@@ -44,8 +52,9 @@ struct Params {
   int64_t* tokens_out; int32_t* parents_out; float* scores_out;
   float* fin_scores_out; int32_t* fin_steps_out; int32_t* fin_beams_out; uint8_t* done_out;
   int32_t* hist_tokens; int32_t* hist_parents; int64_t hist_steps;
-  int32_t B, K, V, n, S;                 // n candidates; S slices per row
-  int32_t groups;                        // maxima published per slice: 1 or 4
+  int32_t B, K, V, n;                    // n candidates
+  int32_t S, cluster_log2;               // slices per row; blocks per sentence
+  uint32_t unit_magic, slice_magic;      // ceil(2^16 / S), ceil(2^32 / S)
   int64_t eos, pad;
   double length_penalty;
   int32_t early_stopping;
@@ -100,18 +109,42 @@ template <> __device__ __forceinline__ void unpack<__half>(const uint4& u, float
   }
 }
 
+// Which of U vectors' elements are at least `least`: bits q and q + 16 (16-bit types: the two halves of word q) or bit q.
+template <typename T, int U> __device__ __forceinline__ uint32_t mask_of(const uint4 (&u)[U], float least) {
+  uint32_t mask = 0;
+  #pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int q = 4 * i + j;
+      if constexpr (sizeof(T) == 4) mask |= __uint_as_float(w[j]) >= least ? 1u << q : 0u;
+      else if constexpr (std::is_same<T, __half>::value)
+        mask |= __hge2_mask(*reinterpret_cast<const __half2*>(&w[j]), __float2half2_rn(least)) & (0x00010001u << q);
+      else
+        mask |= __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[j]), __float2bfloat162_rn(least)) & (0x00010001u << q);
+    }
+  }
+  return mask;
+}
+template <typename T> struct Lowest;     // the lowest finite number: the bound of what can be chosen
+template <> struct Lowest<float> { static constexpr float value = -3.402823466e38f; };
+template <> struct Lowest<__half> { static constexpr float value = -65504.f; };
+template <> struct Lowest<__nv_bfloat16> { static constexpr float value = -3.38953139e38f; };
+
 // A warp's slice of one row: 16-byte vectors [v0, v1) of the row's aligned middle; the first slice also has the
 // elements before it, the last one those behind it (fewer than a vector each, one per lane).
 template <typename T> struct Slice {
   const T* row; const uint4* mid;
   int v0, v1, head, tail, V;             // elements [0, head) and [tail, V) outside the vectors, if this slice has them
-  __device__ __forceinline__ Slice(const T* r, int V_, int part, int S) : row(r), V(V_) {
+  __device__ __forceinline__ Slice(const T* r, int V_, int part, int S, uint32_t magic) : row(r), V(V_) {
     constexpr int N = Pack<T>::N;
     const int mis = (int)(((uintptr_t)r & 15) / sizeof(T));
     const int before = min(mis ? N - mis : 0, V_);
     const int nv = (V_ - before) / N;
     mid = (const uint4*)(r + before);
-    v0 = (int)((int64_t)part * nv / S); v1 = (int)((int64_t)(part + 1) * nv / S);
+    const int each = (S == 1 ? nv : (int)__umulhi((unsigned)nv, magic)) + 1;      // at least nv / S, without a division
+    v0 = (int)min((int64_t)part * each, (int64_t)nv); v1 = min(v0 + each, nv);
     head = part == 0 ? before : 0;
     tail = part == S - 1 ? before + nv * N : V_;
     first = before;
@@ -121,20 +154,32 @@ template <typename T> struct Slice {
   template <typename F> __device__ __forceinline__ void each(int lane, F f) const {
     if (lane < head) f(to_float<T>(row[lane]), lane);
     if (tail + lane < V) f(to_float<T>(row[tail + lane]), tail + lane);
-    for (int v = v0 + lane; v < v1; v += 32) {
-      const uint4 u = __ldg(mid + v);
-      float x[Pack<T>::N];
-      unpack<T>(u, x);
-      #pragma unroll
-      for (int e = 0; e < Pack<T>::N; ++e) f(x[e], first + v * Pack<T>::N + e);
-    }
+    #pragma unroll 1
+    for (int v = v0 + lane; v < v1; v += 32)
+      #pragma unroll 1
+      for (int e = 0; e < Pack<T>::N; ++e) f(to_float<T>(row[first + v * Pack<T>::N + e]), first + v * Pack<T>::N + e);
   }
 };
 
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
 __device__ __forceinline__ double warp_sum(double v) {
   #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// Sum of exponentials of a slice that holds NaN (left out) or +inf (counted): rare, and kept out of the way.
+template <typename T>
+__device__ __noinline__ double careful_sum(const Slice<T>& sl, float most, int lane) {
+  double t = 0.0;
+  sl.each(lane, [&](float x, int) {
+    if (x == x) t += most == INFINITY ? (x == INFINITY ? 1.0 : 0.0) : most > -INFINITY ? (double)fast_exp2((x - most) * kLog2e) : 0.0;
+  });
+  return warp_sum(t);
 }
 
 // Sorted list of the n best keys of a slice, lane i the i-th best (0 = none).
@@ -154,15 +199,13 @@ __device__ __noinline__ uint64_t best_of_slice(const Slice<T>& sl, int beam, int
       if (lane >= n) mine = 0;
     }
   };
-  insert(lane < sl.head ? make_key(beam, to_float<T>(sl.row[lane]), lane) : 0);
-  insert(sl.tail + lane < sl.V ? make_key(beam, to_float<T>(sl.row[sl.tail + lane]), sl.tail + lane) : 0);
-  for (int v = sl.v0; v < sl.v1; v += 32) {
-    const bool in = v + lane < sl.v1;
-    float x[Pack<T>::N];
-    if (in) unpack<T>(__ldg(sl.mid + v + lane), x);
-    #pragma unroll
-    for (int e = 0; e < Pack<T>::N; ++e)
-      insert(in ? make_key(beam, x[e], sl.first + (v + lane) * Pack<T>::N + e) : 0);
+  // the vectors' elements in turn, then those before and behind them
+  #pragma unroll 1
+  for (int i = 0; i < (sl.v1 - sl.v0 + 31) / 32 * Pack<T>::N + 2; ++i) {
+    const int v = sl.v0 + i / Pack<T>::N * 32 + lane, more = i - (sl.v1 - sl.v0 + 31) / 32 * Pack<T>::N;
+    const int token = more < 0 ? sl.first + v * Pack<T>::N + i % Pack<T>::N : more == 0 ? lane : sl.tail + lane;
+    const bool in = more < 0 ? v < sl.v1 : more == 0 ? lane < sl.head : token < sl.V;
+    insert(in ? make_key(beam, to_float<T>(sl.row[token]), token) : 0);
   }
   return mine;
 }
@@ -170,87 +213,144 @@ __device__ __noinline__ uint64_t best_of_slice(const Slice<T>& sl, int beam, int
 struct Shared {
   double usum[MAX_UNITS];
   float umax[MAX_UNITS];
-  float gmax[MAX_GROUPS];
-  float gscore[MAX_GROUPS];
-  Row rows[MAX_BEAMS];
-  Cand found[MAX_SURVIVORS];
-  Cand best[MAX_CAND];
-  uint64_t lists[WARPS][32];
-  Cand heads[WARPS];
-  float bound;
-  int count;
+  alignas(16) float group[THREADS];      // maxima of groups of lanes, a segment's from its first warp's place on
+  float bound[WARPS];                    // found by this warp; the smallest of a segment's holds
+  Row rows[MAX_BEAMS];                   // running rows, in order
+  double inv_length;
+  int counts[MAX_CLUSTER];               // candidates found by each block
+  int found_here, overflow, kept;
+  union {
+    struct {
+      uint64_t found[MAX_FOUND];         // their keys
+      double score[MAX_FOUND + 64];      // scores and keys, one candidate behind the other, padded
+      uint64_t key[MAX_FOUND + 64];
+    };
+    struct {
+      uint64_t lists[WARPS][32];
+      Cand heads[WARPS];
+    };
+  };
+  Cand best[FEW];
 };
 
-// What the step decides from its n best candidates, by one warp: lane i has candidate i (best first).
-__device__ __forceinline__ void decide(const Params& p, const Cand* best, int b, int lane, double length) {
-  const int K = p.K, n = p.n;
-  const unsigned all = 0xffffffffu, below = (1u << lane) - 1;
-  const int64_t at = (int64_t)b * K + lane;
-  const bool valid = lane < n;
-  const double score = valid ? best[lane].score : -INFINITY;
-  const uint64_t key = valid ? best[lane].key : 0;
-  const int token = valid ? key_token(key) : 0, beam = valid ? key_beam(key) : 0;
-  const bool ends = valid && (int64_t)token == p.eos;
-  // the pool: its entries and the ended candidates among the K best, larger first, earlier first among equals
+// The n-th largest of a segment's group maxima: a value that at least n of its elements reach (-inf where too few groups
+// have a finite one).  Every thread brings its own maximum, 2^shift lanes form a group; then threads count
+// for each group how many are above it, and the smallest that fewer than n exceed is the bound.
+__device__ __noinline__ float segment_bound(Shared& sm, float mine, int n, int warp, int lane, int first, int warps, int shift) {
+  if (shift > 0) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+  if (shift > 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+  if (shift > 2) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 4));
+  const int groups = warps * 32 >> shift, at = first * 32, here = warp - first;
+  if ((lane & ((1 << shift) - 1)) == 0) sm.group[at + ((here * 32 + lane) >> shift)] = mine;
+  __syncthreads();
+  // four threads per group, as far as the segment has them (a group each otherwise)
+  const int share = warps > 7 ? 2 : 0, t = here * 32 + lane, g = t >> share;
+  if (here << 5 < groups << share) {
+    const float own = g < groups ? sm.group[at + g] : -INFINITY;
+    int above = 0;
+    const float4* every = (const float4*)(sm.group + at);
+    #pragma unroll 4
+    for (int j = t & ((1 << share) - 1); j < groups / 4; j += 1 << share) {
+      const float4 o = every[j];
+      above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
+    }
+    if (share) {
+      above += __shfl_xor_sync(0xffffffffu, above, 1);
+      above += __shfl_xor_sync(0xffffffffu, above, 2);
+    }
+    const float least = -warp_max(above < n && g < groups ? -own : -INFINITY);
+    if (lane == 0) sm.bound[warp] = least;
+  }
+  __syncthreads();
+  float least = sm.bound[first];
+  for (int i = 1; i << 5 < groups << share; ++i) least = fminf(least, sm.bound[first + i]);
+  return least;
+}
+// lanes per group (their logarithm) so that 33 to 64 groups come out, 32 of a single warp
+__device__ __forceinline__ int group_shift(int warps) { return warps > 8 ? 3 : warps > 4 ? 2 : warps > 2 ? 1 : 0; }
+
+// What the step decides from its n best candidates, best first; a warp each, lane i has candidate i.
+struct Pool { float score; int step, beam; };
+
+// The pool: its entries and the ended candidates among the K best, larger first, earlier first among equals.
+__device__ __forceinline__ void settle(const Params& p, const Cand* best, int b, int lane, const Pool& pool, int64_t pos, double inv_length) {
+  const int K = p.K;
+  const unsigned all = 0xffffffffu;
+  const double score = lane < p.n ? best[lane].score : -INFINITY;
+  const uint64_t key = lane < p.n ? best[lane].key : 0;
+  const bool ends = lane < p.n && (int64_t)key_token(key) == p.eos;
   const bool joins = ends && lane < K && score > -INFINITY;
-  float old = lane < K ? p.fin_scores[at] : -INFINITY;
-  if (!(old == old)) old = -INFINITY;
-  const int old_step = lane < K ? p.fin_steps[at] : 0, old_beam = lane < K ? p.fin_beams[at] : 0;
-  const float fresh = joins ? (float)(score / length) : -INFINITY;
-  const unsigned joining = __ballot_sync(all, joins);
-  int old_rank = 0, new_rank = 0;
-  for (int j = 0; j < K; ++j) {
-    const float o = __shfl_sync(all, old, j);
-    old_rank += o > old || (o == old && j < lane);
-    new_rank += o >= fresh;
+  const unsigned joining = __ballot_sync(all, joins), others = __ballot_sync(all, lane < p.n && !ends);
+  const float highest = (float)__shfl_sync(all, score, __ffs(others) - 1);           // the first that goes on
+  const float old = lane < K && pool.score == pool.score ? pool.score : -INFINITY;
+  const float fresh = joins ? (float)(score * inv_length) : -INFINITY;
+  int old_rank = lane, new_rank = 0;
+  const float next = __shfl_down_sync(all, old, 1);
+  if (joining || __any_sync(all, lane < K - 1 && next > old)) {
+    old_rank = 0;
+    #pragma unroll 1
+    for (int j = 0; j < K; ++j) {
+      const float o = __shfl_sync(all, old, j);
+      old_rank += o > old || (o == old && j < lane);
+      new_rank += o >= fresh;
+    }
+    #pragma unroll 1
+    for (unsigned m = joining; m; m &= m - 1) {
+      const int j = __ffs(m) - 1;
+      const float o = __shfl_sync(all, fresh, j);
+      old_rank += o > old;
+      new_rank += o > fresh || (o == fresh && j < lane);
+    }
   }
-  for (unsigned m = joining; m; m &= m - 1) {
-    const int j = __ffs(m) - 1;
-    const float o = __shfl_sync(all, fresh, j);
-    old_rank += o > old;
-    new_rank += o > fresh || (o == fresh && j < lane);
-  }
-  const int step = (int)(*p.pos);
   if (lane < K && old_rank < K) {
     const int64_t to = (int64_t)b * K + old_rank;
-    p.fin_scores_out[to] = old; p.fin_steps_out[to] = old_step; p.fin_beams_out[to] = old_beam;
+    p.fin_scores_out[to] = old; p.fin_steps_out[to] = pool.step; p.fin_beams_out[to] = pool.beam;
   }
   if (joins && new_rank < K) {
     const int64_t to = (int64_t)b * K + new_rank;
-    p.fin_scores_out[to] = fresh; p.fin_steps_out[to] = step; p.fin_beams_out[to] = beam;
+    p.fin_scores_out[to] = fresh; p.fin_steps_out[to] = (int)pos; p.fin_beams_out[to] = key_beam(key);
   }
-  const unsigned worst_old = __ballot_sync(all, lane < K && old_rank == K - 1);
-  const unsigned worst_new = __ballot_sync(all, joins && new_rank == K - 1);
-  const float worst = worst_old ? __shfl_sync(all, old, __ffs(worst_old) - 1) : __shfl_sync(all, fresh, __ffs(worst_new) - 1);
-  // the K best that go on: one continuation of a beam stays in its place, further ones take the free places in order
-  const int order = __popc(__ballot_sync(all, valid && !ends) & below);
-  const bool on = valid && !ends && order < K;
-  const unsigned goes = __ballot_sync(all, on);
-  const unsigned same = __match_any_sync(all, on ? beam : 64 + lane);
-  const bool further = on && (same & below & goes) != 0;
+  // whoever came last in the pool (one of them is there: K entries and the joining ones fill it)
+  const bool last_old = lane < K && old_rank == K - 1, last_new = joins && new_rank == K - 1;
+  if (last_old || last_new) {
+    const float worst = last_old ? old : fresh;
+    bool full = worst > -INFINITY;
+    if (!p.early_stopping) full = full && (double)worst >= (double)highest * inv_length;
+    p.done_out[b] = full || highest == -INFINITY;
+  }
+}
+
+// The K best that go on: one continuation of a beam stays in its place, further ones take the free places in order.
+__device__ __forceinline__ void go_on(const Params& p, const Cand* best, int b, int lane, int64_t pos) {
+  const int K = p.K;
+  const unsigned all = 0xffffffffu, below = (1u << lane) - 1;
+  const uint64_t key = lane < p.n ? best[lane].key : 0;
+  const int token = key_token(key), beam = key_beam(key);
+  const bool may = lane < p.n && (int64_t)token != p.eos;
+  const int order = __popc(__ballot_sync(all, may) & below);
+  const bool on = may && order < K;
+  unsigned same = 0, used = 0;
+  for (int j = 0; j < K; ++j) {
+    const unsigned those = __ballot_sync(all, on && beam == j);
+    if (beam == j) same = those;
+    used |= those ? 1u << j : 0u;
+  }
+  const bool further = on && (same & below) != 0;
   const unsigned again = __ballot_sync(all, further);
-  const unsigned used = __reduce_or_sync(all, on ? 1u << beam : 0u);
   unsigned open = ~used & ((1u << K) - 1);
   int place = beam;
   if (further) {
+    #pragma unroll 1
     for (int skip = __popc(again & below); skip > 0; --skip) open &= open - 1;
     place = __ffs(open) - 1;
   }
-  const float kept = (float)score;
   if (on && place >= 0) {
     const int64_t to = (int64_t)b * K + place;
-    p.tokens_out[to] = token; p.parents_out[to] = beam; p.scores_out[to] = kept;
-    if (p.hist_tokens && step >= 0 && step < p.hist_steps) {
-      const int64_t h = (int64_t)step * p.B * K + to;
+    p.tokens_out[to] = token; p.parents_out[to] = beam; p.scores_out[to] = (float)best[lane].score;
+    if (p.hist_tokens && pos >= 0 && pos < p.hist_steps) {
+      const int64_t h = pos * p.B * K + to;
       p.hist_tokens[h] = token; p.hist_parents[h] = beam;
     }
-  }
-  const unsigned top = __reduce_max_sync(all, on ? ordered(kept) : 0u);
-  const float highest = unordered(top);
-  if (lane == 0) {
-    bool full = worst > -INFINITY;
-    if (!p.early_stopping) full = full && (double)worst >= (double)highest / length;
-    p.done_out[b] = full || highest == -INFINITY;
   }
 }
 
@@ -259,20 +359,39 @@ __global__ void __launch_bounds__(THREADS, 2)
 step_kernel(const __grid_constant__ Params p) {
   __shared__ Shared sm;
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int b = blockIdx.x / C;
+  const int C = 1 << p.cluster_log2, rank = (int)(blockIdx.x & (C - 1));
+  const int b = blockIdx.x >> p.cluster_log2;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int K = p.K, n = p.n, S = p.S, G = p.groups;
+  const int K = p.K, n = p.n, S = p.S;
   const int64_t at = (int64_t)b * K;
+
+  // the first logits are on their way before anything else is known
+  const int unit = rank * WARPS + warp, row = (int)(unit * p.unit_magic >> 16);
+  const bool owns = row < K;
+  const int k = owns ? row : 0;
+  const Slice<T> sl((const T*)p.logits + (at + k) * p.row_stride, p.V, owns ? unit - row * S : 0, S, p.slice_magic);
+  constexpr int N = Pack<T>::N, U = 4;
+  uint4 u[U];
+  #pragma unroll
+  for (int i = 0; i < U; ++i) {
+    u[i] = make_uint4(Pack<T>::none, Pack<T>::none, Pack<T>::none, Pack<T>::none);
+    if (owns && sl.v0 + lane + 32 * i < sl.v1) u[i] = __ldg(sl.mid + sl.v0 + lane + 32 * i);
+  }
+  const float x_head = owns && lane < sl.head ? to_float<T>(sl.row[lane]) : -INFINITY;
+  const float x_tail = owns && sl.tail + lane < sl.V ? to_float<T>(sl.row[sl.tail + lane]) : -INFINITY;
+  // what the last part needs
+  const int64_t pos = *p.pos;
+  const float run = p.scores[at + k], row_run = warp < K ? p.scores[at + warp] : -INFINITY;
+  Pool pool = {0.f, 0, 0};
+  if (rank == 0 && warp == 1 && lane < K) pool = Pool{p.fin_scores[at + lane], p.fin_steps[at + lane], p.fin_beams[at + lane]};
 
   if (p.done[b]) {                       // the whole cluster: nothing changes any more
     if (rank == 0 && tid < K) {
       p.tokens_out[at + tid] = p.pad; p.parents_out[at + tid] = tid; p.scores_out[at + tid] = p.scores[at + tid];
       p.fin_scores_out[at + tid] = p.fin_scores[at + tid];
       p.fin_steps_out[at + tid] = p.fin_steps[at + tid]; p.fin_beams_out[at + tid] = p.fin_beams[at + tid];
-      const int64_t step = *p.pos;
-      if (p.hist_tokens && step >= 0 && step < p.hist_steps) {
-        p.hist_tokens[(step * p.B + b) * K + tid] = (int32_t)p.pad; p.hist_parents[(step * p.B + b) * K + tid] = tid;
+      if (p.hist_tokens && pos >= 0 && pos < p.hist_steps) {
+        p.hist_tokens[(pos * p.B + b) * K + tid] = (int32_t)p.pad; p.hist_parents[(pos * p.B + b) * K + tid] = tid;
       }
       if (tid == 0) p.done_out[b] = 1;
     }
@@ -280,176 +399,247 @@ step_kernel(const __grid_constant__ Params p) {
   }
 
   // ---- one pass over the logits: maximum and sum of exponentials of a slice
-  const int unit = rank * WARPS + warp, k = unit / S;
-  const bool active = k < K;
-  const Slice<T> sl((const T*)p.logits + (at + (active ? k : 0)) * p.row_stride, p.V, active ? unit % S : 0, S);
+  Shared* lead = cluster.map_shared_rank(&sm, 0);
+  const bool active = owns && run > -INFINITY;
   float m = -INFINITY;
-  if (tid == 0) { sm.count = 0; sm.bound = -INFINITY; }
+  if (tid == 0) { sm.found_here = 0; sm.overflow = 0; sm.kept = 0; }
+  if (tid < MAX_CLUSTER) sm.counts[tid] = 0;
   if (active) {
-    constexpr int N = Pack<T>::N, U = 4;
-    float s = 0.f;
-    auto add = [&](float x) {
-      const float m_new = fmaxf(m, x);
-      if (m_new > -INFINITY) { s = s * fast_exp2((m - m_new) * kLog2e) + fast_exp2((x - m_new) * kLog2e); m = m_new; }
-      else if (!(x == x)) s = x;
-    };
-    if (lane < sl.head) add(to_float<T>(sl.row[lane]));
-    if (sl.tail + lane < sl.V) add(to_float<T>(sl.row[sl.tail + lane]));
-    for (int v = sl.v0 + lane; v < sl.v1; v += 32 * U) {
-      uint4 u[U];
-      #pragma unroll
-      for (int i = 0; i < U; ++i)
-        u[i] = v + 32 * i < sl.v1 ? __ldg(sl.mid + v + 32 * i) : make_uint4(Pack<T>::none, Pack<T>::none, Pack<T>::none, Pack<T>::none);
+    m = fmaxf(fmaxf(x_head, x_tail), -INFINITY);         // (NaN only: -inf)
+    const float edge = m > -INFINITY ? m : 0.f;
+    float s = fast_exp2((x_head - edge) * kLog2e) + fast_exp2((x_tail - edge) * kLog2e);
+    #pragma unroll 1
+    for (int v = sl.v0; v < sl.v1; v += 32 * U) {
       float m_new = m;
       #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        float x[N];
-        unpack<T>(u[i], x);
-        #pragma unroll
-        for (int e = 0; e < N; ++e) m_new = fmaxf(m_new, x[e]);
-      }
+      for (int i = 0; i < U; ++i)
+        if (v + 32 * i < sl.v1) {        // (the same for the whole warp)
+          float x[N];
+          unpack<T>(u[i], x);
+          #pragma unroll
+          for (int e = 0; e < N; e += 4) m_new = fmaxf(m_new, fmaxf(fmaxf(x[e], x[e + 1]), fmaxf(x[e + 2], x[e + 3])));
+        }
       const float ref = m_new > -INFINITY ? m_new : 0.f;
       s *= fast_exp2((m - ref) * kLog2e);
       m = m_new;
+      const bool more = v + 32 * U < sl.v1;
       #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        float x[N];
-        unpack<T>(u[i], x);
-        #pragma unroll
-        for (int e = 0; e < N; ++e) s += fast_exp2((x[e] - ref) * kLog2e);
-      }
+      for (int i = 0; i < U; ++i)
+        if (v + 32 * i < sl.v1) {
+          float x[N];
+          unpack<T>(u[i], x);
+          if (more) {                    // the place is free: the next batch's vector
+            const int next = v + lane + 32 * (U + i);
+            if (next < sl.v1) u[i] = __ldg(sl.mid + next);
+            else u[i] = make_uint4(Pack<T>::none, Pack<T>::none, Pack<T>::none, Pack<T>::none);
+          }
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+          #pragma unroll
+          for (int e = 0; e < N; ++e) part[e & 3] += fast_exp2((x[e] - ref) * kLog2e);
+          s += (part[0] + part[1]) + (part[2] + part[3]);
+        }
     }
-    float gm = m;
-    gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 1));
-    gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
-    gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 4));
-    float wm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 8));
-    wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 16));
+    const float wm = warp_max(m);
     double total;
     if (__any_sync(0xffffffffu, !(s == s) || m == INFINITY)) {      // NaN or +inf among the logits
-      double t = 0.0;
-      sl.each(lane, [&](float x, int) {
-        if (x == x) t += wm == INFINITY ? (x == INFINITY ? 1.0 : 0.0) : wm > -INFINITY ? (double)fast_exp2((x - wm) * kLog2e) : 0.0;
-      });
-      total = warp_sum(t);
+      total = careful_sum<T>(sl, wm, lane);
     } else {
       total = warp_sum(wm > -INFINITY ? (double)(s * fast_exp2((m - wm) * kLog2e)) : 0.0);
     }
-    if (lane < C) {
-      Shared* to = cluster.map_shared_rank(&sm, lane);
-      to->umax[unit] = wm; to->usum[unit] = total;
-      if (G == 1) to->gmax[unit] = wm;
-    }
-    if (G == 4 && (lane & 7) == 0)
-      for (int r = 0; r < C; ++r) cluster.map_shared_rank(&sm, r)->gmax[unit * 4 + lane / 8] = gm;
+    if (lane == 0) { lead->umax[unit] = wm; lead->usum[unit] = total; }
   }
-  cluster.sync();
 
-  // ---- every block: the rows' log-sums, then the bound that n candidates reach
-  if (warp < K) {
-    float rm = -INFINITY;
-    for (int i = lane; i < S; i += 32) rm = fmaxf(rm, sm.umax[warp * S + i]);
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) rm = fmaxf(rm, __shfl_xor_sync(0xffffffffu, rm, o));
-    double t = 0.0;
-    for (int i = lane; i < S; i += 32) {
-      const float um = sm.umax[warp * S + i];
-      if (um > -INFINITY) t += um == rm ? sm.usum[warp * S + i] : sm.usum[warp * S + i] * (double)fast_exp2((um - rm) * kLog2e);
+  // ---- the candidates of this block's segments
+  const int first = active ? max(k * S - rank * WARPS, 0) : warp;                    // the segment's warps
+  const int warps = active ? min((k + 1) * S - rank * WARPS, WARPS) - first : 1;
+  const float least = fmaxf(segment_bound(sm, m, n, warp, lane, first, warps, group_shift(warps)), Lowest<T>::value);
+  const int share = MAX_FOUND >> p.cluster_log2;
+  if (active) {
+    const bool mine = m >= least;
+    const uint32_t flagged = __ballot_sync(0xffffffffu, mine);
+    // the elements among a lane's vectors that reach the bound: bits, then one after the other (small code on purpose:
+    // what runs once per launch pays its way through the instruction cache)
+    auto push = [&](float x, int token) {
+      const int i = atomicAdd(&sm.found_here, 1);
+      if (i < share) lead->found[rank * share + i] = make_key(k, x, token);
+    };
+    if (mine) {
+      if (x_head >= least) push(x_head, lane);
+      if (x_tail >= least) push(x_tail, sl.tail + lane);
     }
-    if (rm == INFINITY) {                // only the slices that have it count
-      t = 0.0;
-      for (int i = lane; i < S; i += 32) if (sm.umax[warp * S + i] == INFINITY) t += sm.usum[warp * S + i];
-    }
-    t = warp_sum(t);
-    if (lane == 0) {
-      const float run = p.scores[at + warp];
-      Row r;
-      r.run = run; r.log_inf = 0.0; r.lse = 0.0;
-      r.state = rm == -INFINITY || !(run > -INFINITY) ? 1 : rm == INFINITY ? 2 : 0;
-      if (r.state == 0) r.lse = (double)rm + log(t);
-      if (r.state == 2) r.log_inf = log(t);
-      sm.rows[warp] = r;
-    }
-  }
-  __syncthreads();
-  const int groups = K * S * G;
-  for (int g = tid; g < groups; g += THREADS)
-    sm.gscore[g] = __double2float_rd(score_of(sm.rows[g / G / S], sm.gmax[g]));
-  __syncthreads();
-  for (int g = tid; g < groups; g += THREADS) {
-    const float mine = sm.gscore[g];
-    int above = 0;
-    for (int j = 0; j < groups; ++j) {
-      const float o = sm.gscore[j];
-      above += o > mine || (o == mine && j < g);
-    }
-    if (above == n - 1) sm.bound = mine;
-  }
-  __syncthreads();
-  const float bound = sm.bound;
-
-  // ---- the candidates that reach the bound
-  bool by_lists = !(bound > -INFINITY);
-  Shared* lead = cluster.map_shared_rank(&sm, 0);
-  if (!by_lists && active) {
-    const Row r = sm.rows[k];
-    if (score_of(r, m) >= (double)bound) {
-      sl.each(lane, [&](float x, int token) {
-        const double s = score_of(r, x);
-        if (s >= (double)bound) {
-          const int i = atomicAdd(&lead->count, 1);
-          if (i < MAX_SURVIVORS) lead->found[i] = Cand{s, make_key(k, x, token)};
+    const bool in_registers = sl.v1 - sl.v0 <= 32 * U;   // the whole slice is still there
+    uint32_t todo = in_registers ? (flagged ? 1u : 0u) : flagged;
+    #pragma unroll 1
+    for (; todo; ) {
+      // from registers, all flagged lanes at once; else the vectors of up to four flagged lanes again, eight lanes for
+      // each, four vectors a lane
+      int base = sl.v0 + lane, stride = 32;
+      bool look = mine;
+      if (!in_registers) {
+        uint32_t t = todo;
+        #pragma unroll 1
+        for (int i = lane >> 3; i > 0; --i) t &= t - 1;
+        look = t != 0;
+        base = sl.v0 + __ffs(t) - 1 + 32 * (lane & 7); stride = 32 * 8;
+        todo &= todo - 1; todo &= todo - 1; todo &= todo - 1; todo &= todo - 1;
+      } else {
+        todo = 0;
+      }
+      #pragma unroll 1
+      for (; __any_sync(0xffffffffu, look && base < sl.v1); base += stride * U) {
+        if (!in_registers) {
+          #pragma unroll
+          for (int i = 0; i < U; ++i)
+            u[i] = look && base + stride * i < sl.v1 ? __ldg(sl.mid + base + stride * i)
+                                                     : make_uint4(Pack<T>::none, Pack<T>::none, Pack<T>::none, Pack<T>::none);
         }
-      });
-    }
-  }
-  cluster.sync();
-  by_lists = by_lists || lead->count > MAX_SURVIVORS;
-
-  if (by_lists) {
-    if (active) sm.lists[warp][lane] = best_of_slice<T>(sl, k, n, lane);
-    cluster.sync();
-    if (rank == 0) {
-      int next = 0;
-      const bool has = tid < K * S;
-      Cand mine{-INFINITY, 0};
-      auto take = [&]() {
-        mine.key = next < n ? cluster.map_shared_rank(&sm, tid / WARPS)->lists[tid % WARPS][next] : 0;
-        mine.score = mine.key ? score_of(sm.rows[tid / S], key_logit(mine.key)) : -INFINITY;
-      };
-      if (has) take();
-      for (int i = 0; i < n; ++i) {
-        Cand top = mine;
-        #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const double os = __shfl_xor_sync(0xffffffffu, top.score, o);
-          const uint64_t ok = __shfl_xor_sync(0xffffffffu, top.key, o);
-          if (better(os, ok, top.score, top.key)) { top.score = os; top.key = ok; }
+        uint32_t mask = look ? mask_of<T, U>(u, least) : 0;
+        #pragma unroll 1
+        for (; mask; mask &= mask - 1) {
+          const int bit = __ffs(mask) - 1, q = bit & 15, i = q >> 2, e = N == 8 ? 2 * (q & 3) + (bit >> 4) : q & 3;
+          uint4 w = u[0];
+          #pragma unroll
+          for (int j = 1; j < U; ++j) if (i == j) w = u[j];
+          float x[N], found = 0.f;
+          unpack<T>(w, x);
+          #pragma unroll
+          for (int j = 0; j < N; ++j) if (e == j) found = x[j];
+          push(found, sl.first + (base + stride * i) * N + e);
         }
-        if (lane == 0) sm.heads[warp] = top;
-        __syncthreads();
-        top = sm.heads[0];
-        #pragma unroll
-        for (int w = 1; w < WARPS; ++w) if (better(sm.heads[w].score, sm.heads[w].key, top.score, top.key)) top = sm.heads[w];
-        if (tid == 0) sm.best[i] = top;
-        if (mine.key && mine.key == top.key) { ++next; take(); }
-        __syncthreads();
       }
     }
-  } else if (rank == 0) {
-    const int found = sm.count;
-    for (int i = tid; i < found; i += THREADS) {
-      const Cand mine = sm.found[i];
-      int above = 0;
-      for (int j = 0; j < found; ++j) above += better(sm.found[j].score, sm.found[j].key, mine.score, mine.key);
-      if (above < n) sm.best[above] = mine;
+  }
+  __syncthreads();
+  if (tid == 0) lead->counts[rank] = sm.found_here;
+  cluster.sync();
+
+  // ---- the first block: log-sums, scores, the n best
+  if (rank == 0) {
+    if (warp < K) {
+      float most = -INFINITY;
+      #pragma unroll 1
+      for (int i = row_run > -INFINITY ? lane : S; i < S; i += 32) most = fmaxf(most, sm.umax[warp * S + i]);
+      most = warp_max(most);
+      double sum = 0.0;
+      #pragma unroll 1
+      for (int i = most > -INFINITY ? lane : S; i < S; i += 32) {
+        const float um = sm.umax[warp * S + i];
+        if (um == most) sum += sm.usum[warp * S + i];
+        else if (most < INFINITY && um > -INFINITY) sum += sm.usum[warp * S + i] * (double)fast_exp2((um - most) * kLog2e);
+      }
+      sum = log(warp_sum(sum));
+      if (lane == 0) sm.rows[warp] = Row{row_run, (double)most + sum, sum, !(most > -INFINITY) ? 1 : most == INFINITY ? 2 : 0};
+    }
+    if (warp == WARPS - 1 && lane == 1) {                // (K = 16: this warp has a row as well)
+      const double steps = (double)(pos + 1);
+      sm.inv_length = p.length_penalty == 1.0 ? 1.0 / steps : p.length_penalty == 0.0 ? 1.0 : pow(steps, -p.length_penalty);
+    }
+    int total = 0, before = 0;
+    bool fits = true;
+    #pragma unroll
+    for (int r = 0; r < MAX_CLUSTER; ++r) {
+      const int c = sm.counts[r];
+      fits = fits && c <= share;
+      before += r < (warp & (C - 1)) ? c : 0;
+      total += c;
     }
     __syncthreads();
+    int valid = 0;
+    if (fits) {
+      // warps take the blocks' lists in turn
+      const int r = warp & (C - 1), step = WARPS * 32 >> p.cluster_log2;
+      #pragma unroll 1
+      for (int i = (warp >> p.cluster_log2) * 32 + lane; i < sm.counts[r]; i += step) {
+        const uint64_t key = sm.found[r * share + i];
+        const double score = score_of(sm.rows[key_beam(key)], key_logit(key));
+        sm.score[before + i] = score; sm.key[before + i] = key;
+        valid += score > -INFINITY;
+      }
+    }
+    if (tid < 64 && fits) { sm.score[total + tid] = -INFINITY; sm.key[total + tid] = 0; }
+    valid = __reduce_add_sync(0xffffffffu, valid);
+    if (lane == 0 && valid) atomicAdd(&sm.kept, valid);
+    __syncthreads();
+    bool done = fits && sm.kept >= n;
+    __syncthreads();
+    int count = total;
+    if (done && total > FEW) {
+      // many: the same bound again, over the candidates (thread t has candidates t / 8 + 64 * (t % 8) and 512 further on)
+      const int i0 = (tid >> 3) + 64 * (tid & 7), i1 = i0 + THREADS;
+      const float f0 = i0 < total ? __double2float_rd(sm.score[i0]) : -INFINITY;
+      const float f1 = i1 < total ? __double2float_rd(sm.score[i1]) : -INFINITY;
+      if (tid == 0) sm.kept = 0;
+      const float least = segment_bound(sm, fmaxf(f0, f1), n, warp, lane, 0, WARPS, 3);
+      if (f0 >= least && f0 > -INFINITY) { const int i = atomicAdd(&sm.kept, 1); if (i < FEW) sm.best[i] = Cand{sm.score[i0], sm.key[i0]}; }
+      if (f1 >= least && f1 > -INFINITY) { const int i = atomicAdd(&sm.kept, 1); if (i < FEW) sm.best[i] = Cand{sm.score[i1], sm.key[i1]}; }
+      __syncthreads();
+      count = sm.kept;
+      done = count >= n && count <= FEW;
+      if (done && tid < FEW + 64) {
+        const Cand c = tid < count ? sm.best[tid] : Cand{-INFINITY, 0};
+        sm.score[tid] = c.score; sm.key[tid] = c.key;
+      }
+      __syncthreads();
+    }
+    if (done) {
+      asm volatile("barrier.cluster.arrive.relaxed.aligned;");               // the others may go: nothing more reaches them
+      // 4 to 16 threads count for each of the candidates, four comparisons at a time
+      const int team_log2 = count <= 32 ? 4 : count <= 64 ? 3 : 2, team = 1 << team_log2, i = tid >> team_log2;
+      if (i < count) {
+        const double score = sm.score[i];
+        const uint64_t key = sm.key[i];
+        int above = 0;
+        #pragma unroll 1
+        for (int j = tid & (team - 1); j < count; j += 4 * team) {
+          #pragma unroll
+          for (int o = 0; o < 4; ++o) above += better(sm.score[j + o * team], sm.key[j + o * team], score, key);
+        }
+        // (teams that share a warp are all in or all out only up to the last one: only its lanes take part)
+        const unsigned lanes = ((1u << team) - 1) << (lane & -team);
+        for (int o = 1; o < team; o <<= 1) above += __shfl_xor_sync(lanes, above, o);
+        if ((tid & (team - 1)) == 0 && above < n) sm.best[above] = Cand{score, key};
+      }
+      __syncthreads();
+      if (warp == 0) go_on(p, sm.best, b, lane, pos);
+      if (warp == 1) settle(p, sm.best, b, lane, pool, pos, sm.inv_length);
+      return;
+    }
+    if (tid < C) cluster.map_shared_rank(&sm, tid)->overflow = 1;
   }
-  if (rank == 0 && warp == 0) {
-    const double steps = (double)(*p.pos + 1);
-    const double length = p.length_penalty == 1.0 ? steps : p.length_penalty == 0.0 ? 1.0 : pow(steps, p.length_penalty);
-    decide(p, sm.best, b, lane, length);
+  cluster.sync();
+  if (!sm.overflow) return;
+
+  // ---- too few or too many candidates: a sorted list per slice of every row, merged by the first block
+  if (owns) sm.lists[warp][lane] = best_of_slice<T>(sl, k, n, lane);
+  cluster.sync();
+  if (rank == 0) {
+    int next = 0;
+    Cand mine{-INFINITY, 0};
+    auto take = [&]() {
+      mine.key = next < n ? cluster.map_shared_rank(&sm, tid / WARPS)->lists[tid % WARPS][next] : 0;
+      mine.score = mine.key ? score_of(sm.rows[tid / S], key_logit(mine.key)) : -INFINITY;
+    };
+    if (tid < K * S) take();
+    #pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      Cand top = mine;
+      #pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const double os = __shfl_xor_sync(0xffffffffu, top.score, o);
+        const uint64_t ok = __shfl_xor_sync(0xffffffffu, top.key, o);
+        if (better(os, ok, top.score, top.key)) { top.score = os; top.key = ok; }
+      }
+      if (lane == 0) sm.heads[warp] = top;
+      __syncthreads();
+      top = sm.heads[0];
+      #pragma unroll 1
+      for (int w = 1; w < WARPS; ++w) if (better(sm.heads[w].score, sm.heads[w].key, top.score, top.key)) top = sm.heads[w];
+      if (tid == 0) sm.best[i] = top;
+      if (mine.key && mine.key == top.key) { ++next; take(); }
+      __syncthreads();
+    }
+    if (warp == 0) go_on(p, sm.best, b, lane, pos);
+    if (warp == 1) settle(p, sm.best, b, lane, pool, pos, sm.inv_length);
   }
   cluster.sync();                        // nobody leaves while its shared memory is read
 }
@@ -561,18 +751,29 @@ sequences_kernel(const __grid_constant__ SequenceParams p) {
   }
 }
 
-static int cluster_blocks(int B) {
-  // A block per multiprocessor and a half keeps the whole batch resident; more blocks per sentence shorten its pass.
-  int C = MAX_CLUSTER;
-  while (C > 1 && (long long)B * C > 2 * 148) C /= 2;
+static int cluster_blocks(int B, int K, int64_t bytes) {
+  // Two blocks per multiprocessor keep the whole batch resident; more blocks per sentence shorten its pass, 16 only where
+  // a slice would not fit a warp's registers with 8 (a sentence of 4 x 32128 16-bit logits: 7.9 us with 8, 8.5 with 16;
+  // of 16 x 65537 float32: 26.7 and 21.6).  A beam has two warps at least, for the number of groups that its bound is
+  // taken from.
+  int C = bytes > 8 * WARPS * 32 * 4 * 16 ? 16 : 8;
+  while (C > (K > 8 ? 2 : 1) && (long long)B * C > (C == 16 ? 148 : 2 * 148)) C /= 2;
   return C;
 }
 
 template <typename T>
 static int launch_step(Params p, cudaStream_t stream) {
-  const int C = cluster_blocks(p.B);
+  static std::atomic<bool> wide[64];     // per device: clusters of 16 are allowed for this kernel (setting it twice is harmless)
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return T5B_ERR_LAUNCH;
+  if (!wide[dev]) {
+    if (cudaFuncSetAttribute(step_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return T5B_ERR_LAUNCH;
+    wide[dev] = true;
+  }
+  const int C = cluster_blocks(p.B, p.K, (int64_t)p.K * p.V * sizeof(T));
+  for (p.cluster_log2 = 0; 1 << p.cluster_log2 < C;) ++p.cluster_log2;
   p.S = C * WARPS / p.K;
-  p.groups = C * WARPS <= 32 ? 4 : 1;
+  p.unit_magic = (65536u + p.S - 1) / p.S; p.slice_magic = (uint32_t)(((1ull << 32) + p.S - 1) / p.S);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.B * C)); cfg.blockDim = dim3(THREADS); cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -607,7 +808,7 @@ extern "C" int t5b_beam_search_step(const t5b_beam_step_args* a, void* stream) {
   p.fin_scores_out = a->finished_scores_out; p.fin_steps_out = a->finished_steps_out;
   p.fin_beams_out = a->finished_beams_out; p.done_out = a->done_out;
   p.hist_tokens = a->history_tokens; p.hist_parents = a->history_parents; p.hist_steps = a->history_steps;
-  p.B = a->B; p.K = a->num_beams; p.V = a->vocab; p.n = 2 * a->num_beams; p.S = 1; p.groups = 1;
+  p.B = a->B; p.K = a->num_beams; p.V = a->vocab; p.n = 2 * a->num_beams;
   p.eos = a->eos_token_id; p.pad = a->pad_token_id;
   p.length_penalty = a->length_penalty; p.early_stopping = a->early_stopping;
   cudaStream_t st = (cudaStream_t)stream;
