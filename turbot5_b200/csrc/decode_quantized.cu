@@ -10,15 +10,19 @@
 //
 //   * S^T = K Q^T: the keys are the rows of the product.  A lane's 16 bytes of a key are four k-steps of the A operand
 //     as they stand (the order of the head dim inside a k-step is free, the queries are read in the same order).
-//   * O^T = V^T P^T: the head dim is the rows.  A byte permute joins two keys' bytes to pairs along the key dim.
+//   * O^T = V^T P^T: the head dim is the rows.  A byte permute joins two keys' bytes to pairs along the key dim.  Which
+//     key is which row of a 16-key tile is free as well: the order is such that reading values has no bank conflicts.
 //   * P^T comes out of S^T's registers by one 8x8 transpose of 16-bit pairs.
-//   * fp16 products of e4m3 numbers are exact in float32; q is scaled to 1 by a power of two.  P is carried as
-//     hi + lo in two columns: with up to four rows the eight columns hold each row twice, with up to eight rows the
-//     product is issued twice, so P keeps 22 bits and the result is as exact as float32 weights would make it.
+//   * fp16 products of e4m3 numbers are exact in float32; q is scaled to 1 by a power of two.  P is carried as hi + lo:
+//     with up to four rows, row r has columns 2r and 2r + 1 of the product, one for each half (a lane then makes the
+//     weights of one row only); with up to eight rows the product is issued twice.  P keeps 22 bits, so the result is
+//     as exact as float32 weights would make it.
 //
-// A warp owns blocks of 64 keys (so a block has one scale), with its own running maximum and sum; warps merge in shared
-// memory, the blocks of a (batch, head) that share a long cache form a cluster and merge through distributed shared
-// memory: no workspace, no counters, no second launch.
+// A warp works on items of 32 or 64 keys of one block of 64 (so an item has one scale), with its own running maximum and
+// sum and its own ring of stages in shared memory that asynchronous copies fill ahead (registers alone held too little in
+// flight: 206 us instead of TIME for 1.07 GB).  Warps merge in shared memory, the blocks of a (batch, head) that share a long cache form a cluster and merge through distributed
+// shared memory: no workspace, no counters, no second launch.  The bias is looked up for items within the largest
+// distance of a query only, from a table of the item's distances that the warp makes for itself.
 //
 // Semantics: the cached step of T5Attention.forward (src/turbot5/model/attentions.py:198,229-234), the merge rule of
 // src/turbot5/ops/flash_decoding.py:47-55, as in decode.cu.
@@ -26,15 +30,33 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 namespace cg = cooperative_groups;
 
 namespace t5b {
 namespace decq {
 
 constexpr int BLOCK = T5B_CACHE_BLOCK;
-constexpr int WARPS = 4;
-constexpr int THREADS = WARPS * 32;
-constexpr int MAX_CLUSTER = 8;
+constexpr int MAX_CLUSTER = 16;          // more than 8 is beyond what every GPU has to offer, but not this one
+#ifndef DQ_SUB
+#define DQ_SUB 2
+#endif
+#ifndef DQ_STAGES
+#define DQ_STAGES 3
+#endif
+#ifndef DQ_MINW
+#define DQ_MINW 16
+#endif
+
+// 16-key tiles of an item, and how its stages lie in shared memory: keys, values, two scales
+template <int D> struct Ring {
+  static constexpr int SUB = D == 128 ? 2 : D == 64 ? DQ_SUB : 4;
+  static constexpr int STAGES = D == 128 ? 2 : DQ_STAGES;
+  static constexpr int ITEM = SUB * 16;
+  static constexpr int BYTES = 2 * ITEM * D + 16;
+  static constexpr int WARP_BYTES = STAGES * BYTES;
+};
 
 struct Params {
   const void* q; const uint8_t* k; const uint8_t* v; const float* k_scale; const float* v_scale; void* out;
@@ -44,14 +66,14 @@ struct Params {
   int64_t ks_stride_b, ks_stride_h, vs_stride_b, vs_stride_h;
   int64_t o_stride_b, o_stride_h, o_stride_m;
   int64_t table_stride0;
-  int32_t table_dtype, B, H, M, N, causal, q_pos_offset, row_groups;
+  int32_t table_dtype, B, H, M, N, causal, q_pos_offset, row_groups, q_aligned;
   float scale_log2;
 };
 
-__device__ __forceinline__ uint32_t half2_of_e4m3x2(uint32_t two_bytes) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two_bytes));
-  return h;
+// four e4m3 numbers -> two fp16 pairs
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -67,21 +89,30 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   return y;
 }
 
-// BYTES consecutive bytes of a row into words, streaming
-template <int BYTES> __device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
+__device__ __forceinline__ void copy_async16(uint32_t to, const void* from, bool in) {   // zeros where `in` is false
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// BYTES consecutive bytes of a row in shared memory into words
+template <int BYTES> __device__ __forceinline__ void read_bytes(const uint8_t* p, uint32_t* w) {
   if constexpr (BYTES == 2) {
-    uint16_t t;
-    asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(t) : "l"(p));
-    w[0] = t;
+    w[0] = *(const uint16_t*)p;
   } else if constexpr (BYTES == 4) {
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+    w[0] = *(const uint32_t*)p;
   } else if constexpr (BYTES == 8) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    const uint2 u = *(const uint2*)p;
+    w[0] = u.x; w[1] = u.y;
   } else {
     #pragma unroll
-    for (int i = 0; i < BYTES / 16; ++i)
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3]) : "l"(p + 64 * i));
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 u = *(const uint4*)(p + 64 * i);
+      w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+    }
   }
 }
 
@@ -90,51 +121,120 @@ template <int D> __device__ __forceinline__ int dim_of(int c, int j, int e) {
   return D == 128 ? j / 4 * 64 + 16 * c + 4 * (j & 3) + e : D / 4 * c + 4 * j + e;
 }
 
-// TILES 1: up to four rows, hi and lo of P in the columns of one product.  TILES 2: up to eight rows, two products.
-template <typename T, int D, int TILES>
-__global__ void __launch_bounds__(THREADS)
+// TILES 1: up to four rows, each with two columns of the products (hi and lo of its weights).  TILES 2: up to eight rows,
+// a column each, the second product twice.
+template <typename T, int D, int TILES, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, TILES == 1 && D <= 64 ? DQ_MINW / WARPS : 1)
 decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant__ BucketSpec spec) {
+  using R = Ring<D>;
+  constexpr int THREADS = WARPS * 32;
   constexpr int ROWS = 4 * TILES;
   constexpr int KSTEPS = D / 16;         // k-steps of S^T, 16-row tiles of O^T
   constexpr int KB = D / 4, VB = D / 8;  // bytes of a key / value row that a lane holds
   constexpr int KW = KB / 4, VW = (VB + 3) / 4;
-  constexpr int SUB = D == 128 ? 2 : 4;  // 16-key tiles whose loads are in flight together
-  extern __shared__ float lut[];
-  __shared__ float sm_m[WARPS][8], sm_l[WARPS][8];
-  __shared__ float sm_o[WARPS][ROWS][D];
+  constexpr int SUB = R::SUB, ITEM = R::ITEM, STAGES = R::STAGES;
+  constexpr int COLS = TILES;            // columns of this lane that are rows of their own
+  constexpr int NEAR = ITEM + ROWS;      // distances between an item's keys and the rows
+  static_assert(ROWS * D * 4 <= R::WARP_BYTES, "a warp's result takes the place of its ring");
+  extern __shared__ __align__(16) uint8_t rings[];
+  __shared__ float near_bias[WARPS][NEAR];
+  __shared__ float sm_m[WARPS][ROWS], sm_l[WARPS][ROWS];
   __shared__ float out_m[ROWS], out_l[ROWS], out_o[ROWS][D];
 
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int C = gridDim.x, rank = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
-  const int h = blockIdx.y, b = blockIdx.z / p.row_groups, m0 = blockIdx.z % p.row_groups * ROWS;
-  const int kv_len = p.seqlens_k ? min(max(p.seqlens_k[b], 0), p.N) : p.N;
+  const int key_of_g = (g >> 1) + 4 * (g & 1);             // the key of row g of a tile; row g + 8: 8 more
+  const int h = blockIdx.y, b = p.row_groups == 1 ? blockIdx.z : blockIdx.z / p.row_groups;
+  const int m0 = (blockIdx.z - b * p.row_groups) * ROWS;
+  // ---- everything that waits for nothing is requested first: the length, the queries (column n of the products is row
+  // m0 + n / 2 or, with TILES 2, m0 + n), the head's bias table (lane i has bucket i) and the buckets' first distances
+  const int given_len = p.seqlens_k ? p.seqlens_k[b] : p.N;
+  uint2 raw[KSTEPS];                     // four elements each
+  {
+    const int row = m0 + (TILES == 1 ? g >> 1 : g);
+    const T* qp = (const T*)p.q + (int64_t)b * p.q_stride_b + (int64_t)h * p.q_stride_h + (int64_t)(row < p.M ? row : 0) * p.q_stride_m;
+    #pragma unroll
+    for (int j = 0; j < KSTEPS; ++j) {
+      raw[j] = make_uint2(0, 0);
+      if (row < p.M) {
+        const T* at = qp + dim_of<D>(c, j, 0);
+        if (p.q_aligned) {
+          raw[j] = __ldg((const uint2*)at);
+        } else {
+          const uint16_t* e = (const uint16_t*)at;
+          raw[j] = make_uint2(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16);
+        }
+      }
+    }
+  }
+  const bool has_bias = p.table != nullptr;
+  const int buckets = spec.bidirectional ? 2 * spec.n_side : spec.n_side;
+  float lane_bias = 0.f;
+  int lane_first = 1 << 30;
+  if (has_bias && buckets <= 32) {
+    if (lane < buckets) lane_bias = load_table(p.table, p.table_dtype, (int64_t)lane * p.table_stride0 + h);
+    if (lane < spec.n_first) lane_first = spec.first[lane];
+  }
+  auto bias_of = [&](int delta) -> float {               // by whole warps
+    if (buckets > 32) return kLog2e * load_table(p.table, p.table_dtype, (int64_t)bucket_of_delta(spec, delta) * p.table_stride0 + h);
+    const int d = min(spec.bidirectional ? abs(delta) : max(-delta, 0), spec.max_distance);
+    int n = 0;                                           // first distances that d reaches: a search over the lanes
+    #pragma unroll
+    for (int half = 16; half > 0; half >>= 1) n += __shfl_sync(0xffffffffu, lane_first, n + half - 1) <= d ? half : 0;
+    return kLog2e * __shfl_sync(0xffffffffu, lane_bias, n + (spec.bidirectional && delta > 0 ? spec.n_side : 0));
+  };
+  const int kv_len = min(max(given_len, 0), p.N);
   const int qoff = p.q_pos_offset >= 0 ? p.q_pos_offset : kv_len - p.M;
   const int md = spec.max_distance;
-  const bool has_bias = p.table != nullptr;
-  if (has_bias) {
-    for (int i = tid; i < 2 * md + 1; i += THREADS)
-      lut[i] = load_table(p.table, p.table_dtype, (int64_t)bucket_of_delta(spec, i - md) * p.table_stride0 + h) * kLog2e;
-    __syncthreads();
-  }
+  // keys behind the last visible one of the last row are never touched
+  const int first_pos = qoff + m0, last_pos = qoff + min(m0 + ROWS, p.M) - 1;
+  const int n_end = p.causal ? min(kv_len, max(last_pos + 1, 0)) : kv_len;
+  const int items = (n_end + ITEM - 1) / ITEM, step = C * WARPS;
 
-  // ---- queries: column n of the products is row m0 + n (TILES 2) or m0 + n % 4 (TILES 1), scaled to at most 1
+  uint8_t* ring = rings + warp * R::WARP_BYTES;
+  const uint8_t* kb = p.k + (int64_t)b * p.k_stride_b + (int64_t)h * p.k_stride_h + lane * 16;
+  const uint8_t* vb = p.v + (int64_t)b * p.v_stride_b + (int64_t)h * p.v_stride_h + lane * 16;
+  const float* ks = p.k_scale + (int64_t)b * p.ks_stride_b + (int64_t)h * p.ks_stride_h;
+  const float* vs = p.v_scale + (int64_t)b * p.vs_stride_b + (int64_t)h * p.vs_stride_h;
+  // an item's rows lie one behind the other: 16 bytes a lane; zeros behind the last key
+  auto request = [&](int it, int stage) {
+    if (it < items) {
+      const int n0 = it * ITEM;
+      const int64_t from = (int64_t)n0 * D;
+      const uint32_t to = smem_u32(ring + stage * R::BYTES) + lane * 16;
+      const int bytes = (n_end - n0) * D - lane * 16;      // of this lane's first piece on
+      #pragma unroll
+      for (int i = 0; i < (ITEM * D + 511) / 512; ++i)
+        if (ITEM * D % 512 == 0 || lane * 16 + i * 512 < ITEM * D) {
+          const bool in = i * 512 < bytes;
+          copy_async16(to + i * 512, kb + (in ? from + i * 512 : 0), in);
+          copy_async16(to + ITEM * D + i * 512, vb + (in ? from + i * 512 : 0), in);
+        }
+      if (lane < 2) copy_async4(smem_u32(ring + stage * R::BYTES + 2 * ITEM * D) + 4 * lane, (lane ? vs : ks) + n0 / BLOCK);
+    }
+    copy_commit();
+  };
+  int it = rank * WARPS + warp;
+  #pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) request(it + i * step, i);
+
+  // ---- queries, scaled to at most 1
   uint32_t qf[KSTEPS][2];
-  float col_scale[2];                    // of this lane's columns 2c and 2c + 1
-  int col_pos[2];
+  float col_scale[COLS];                 // of this lane's rows: c (TILES 1) or 2c and 2c + 1
+  int col_pos[COLS];
   {
-    const int row = m0 + (TILES == 1 ? (g & 3) : g);
-    const bool in = row < p.M;
-    const T* qp = (const T*)p.q + (int64_t)b * p.q_stride_b + (int64_t)h * p.q_stride_h + (int64_t)(in ? row : 0) * p.q_stride_m;
     float x[KSTEPS][4], most = 0.f;
     #pragma unroll
-    for (int j = 0; j < KSTEPS; ++j)
+    for (int j = 0; j < KSTEPS; ++j) {
+      const T* t = reinterpret_cast<const T*>(&raw[j]);
       #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[j][e] = in ? to_float<T>(qp[dim_of<D>(c, j, e)]) : 0.f;
+        x[j][e] = to_float<T>(t[e]);
         most = fmaxf(most, fabsf(x[j][e]));
       }
+    }
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     // a power of two at or below the largest element (1 where that is 0, tiny or not finite)
@@ -147,14 +247,22 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
       qf[j][1] = pack_half2(x[j][2] * inv, x[j][3] * inv);
     }
     #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int col = 2 * c + i, r = TILES == 1 ? col & 3 : col;
-      col_scale[i] = __shfl_sync(0xffffffffu, unit, r * 4) * p.scale_log2;
-      col_pos[i] = qoff + m0 + r;
+    for (int i = 0; i < COLS; ++i) {
+      const int r = TILES == 1 ? c : 2 * c + i;
+      col_scale[i] = __shfl_sync(0xffffffffu, unit, (TILES == 1 ? 2 * r : r) * 4) * p.scale_log2;
+      col_pos[i] = first_pos + r;
     }
   }
 
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  float bias_before = 0.f, bias_after = 0.f;
+  if (has_bias) {
+    bias_before = bias_of(-md);
+    bias_after = bias_of(md);
+  }
+
+  float m_run[COLS], l_run[COLS];
+  #pragma unroll
+  for (int i = 0; i < COLS; ++i) { m_run[i] = -INFINITY; l_run[i] = 0.f; }
   float acc[TILES][KSTEPS][4];
   #pragma unroll
   for (int t = 0; t < TILES; ++t)
@@ -163,148 +271,156 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
       #pragma unroll
       for (int e = 0; e < 4; ++e) acc[t][i][e] = 0.f;
 
-  const uint8_t* kb = p.k + (int64_t)b * p.k_stride_b + (int64_t)h * p.k_stride_h + (D == 128 ? 16 : KB) * c;
-  const uint8_t* vb = p.v + (int64_t)b * p.v_stride_b + (int64_t)h * p.v_stride_h + VB * g;
-  const float* ks = p.k_scale + (int64_t)b * p.ks_stride_b + (int64_t)h * p.ks_stride_h;
-  const float* vs = p.v_scale + (int64_t)b * p.vs_stride_b + (int64_t)h * p.vs_stride_h;
-  // keys behind the last visible one of the last row are never touched
-  const int last_pos = qoff + min(m0 + ROWS, p.M) - 1;
-  const int n_end = p.causal ? min(kv_len, max(last_pos + 1, 0)) : kv_len;
-  const int blocks = (n_end + BLOCK - 1) / BLOCK;
-
-  for (int blk = rank * WARPS + warp; blk < blocks; blk += C * WARPS) {
-    const float k_scale = __ldg(ks + blk), v_scale = __ldg(vs + blk);
-    const int n0 = blk * BLOCK;
-    const bool whole = n0 + BLOCK <= n_end && (!p.causal || n0 + BLOCK - 1 <= qoff + m0);
-    // every key of the block beyond the largest distance from every row: one bias value
-    const bool before = n0 + BLOCK - 1 - (qoff + m0) <= -md;
-    const bool far = has_bias && (before || n0 - last_pos >= md);
-    const float far_bias = far ? lut[before ? 0 : 2 * md] : 0.f;
+  int stage = 0;
+  #pragma unroll 1
+  for (; it < items; it += step) {
+    copy_wait<STAGES - 2>();
+    __syncwarp();
+    request(it + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);    // (the stage that the last turn has read)
+    const uint8_t* keys = ring + stage * R::BYTES;
+    const uint8_t* values = keys + ITEM * D;
+    const float k_scale = *(const float*)(values + ITEM * D), v_scale = *(const float*)(values + ITEM * D + 4);
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+    const int n0 = it * ITEM;
+    const bool whole = n0 + ITEM <= n_end && (!p.causal || n0 + ITEM - 1 <= first_pos);
+    // ---- scores of the item's keys
+    float s[SUB][2 * COLS];              // this lane's two keys of each tile, this lane's rows
     #pragma unroll
-    for (int half = 0; half < 4 / SUB; ++half) {
-      const int nb = n0 + half * SUB * 16;
-      if (half > 0 && nb >= n_end) break;
-      uint32_t kw[SUB][2][KW], vw[SUB][4][VW];
+    for (int t = 0; t < SUB; ++t) {
+      uint32_t k0[KW], k1[KW];
+      const uint8_t* at = keys + (t * 16 + key_of_g) * D + (D == 128 ? 16 : KB) * c;
+      read_bytes<KB>(at, k0);
+      read_bytes<KB>(at + 8 * D, k1);
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
       #pragma unroll
-      for (int t = 0; t < SUB; ++t)
-        #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int n = nb + t * 16 + g + 8 * i;
-          #pragma unroll
-          for (int w = 0; w < KW; ++w) kw[t][i][w] = 0;
-          if (whole || n < n_end) load_bytes<KB>(kb + (int64_t)n * D, kw[t][i]);
-        }
-      #pragma unroll
-      for (int t = 0; t < SUB; ++t)
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = nb + t * 16 + 2 * c + (i & 1) + 8 * (i >> 1);
-          #pragma unroll
-          for (int w = 0; w < VW; ++w) vw[t][i][w] = 0;
-          if (whole || n < n_end) load_bytes<VB>(vb + (int64_t)n * D, vw[t][i]);
-        }
-      // ---- scores of SUB x 16 keys
-      float s[SUB][4];
-      #pragma unroll
-      for (int t = 0; t < SUB; ++t) {
-        #pragma unroll
-        for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
-        #pragma unroll
-        for (int j = 0; j < KSTEPS; ++j)
-          mma_16816(s[t], half2_of_e4m3x2(kw[t][0][j] & 0xffffu), half2_of_e4m3x2(kw[t][1][j] & 0xffffu),
-                    half2_of_e4m3x2(kw[t][0][j] >> 16), half2_of_e4m3x2(kw[t][1][j] >> 16), qf[j][0], qf[j][1]);
-      }
-      const float f0 = col_scale[0] * k_scale, f1 = col_scale[1] * k_scale;
-      float mx[2] = {-INFINITY, -INFINITY};
-      #pragma unroll
-      for (int t = 0; t < SUB; ++t)
-        #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = nb + t * 16 + g + 8 * (e >> 1);
-          float bias = far_bias;
-          if (has_bias && !far) bias = lut[min(max(n - col_pos[e & 1] + md, 0), 2 * md)];
-          s[t][e] = fmaf(s[t][e], e & 1 ? f1 : f0, bias);
-          if (!whole && (n >= n_end || (p.causal && n > col_pos[e & 1]))) s[t][e] = -INFINITY;
-          mx[e & 1] = fmaxf(mx[e & 1], s[t][e]);
-        }
-      // ---- running maximum, weights
-      float alpha[2], ref[2];
-      #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 4));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 8));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 16));
-        const float m_new = fmaxf(m_run[i], mx[i]);
-        ref[i] = m_new == -INFINITY ? 0.f : m_new;
-        alpha[i] = fast_exp2(m_run[i] - ref[i]);
-        m_run[i] = m_new;
-        l_run[i] *= alpha[i];
-      }
-      float part[TILES][KSTEPS][4];
-      #pragma unroll
-      for (int t = 0; t < TILES; ++t)
-        #pragma unroll
-        for (int i = 0; i < KSTEPS; ++i)
-          #pragma unroll
-          for (int e = 0; e < 4; ++e) part[t][i][e] = 0.f;
-      #pragma unroll
-      for (int t = 0; t < SUB; ++t) {
-        float w[4], lo[4];
-        #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = fast_exp2(s[t][e] - ref[e & 1]);
-          l_run[e & 1] += w[e];
-          lo[e] = w[e] - __half2float(__float2half_rn(w[e]));
-        }
-        uint32_t b0, b1, c0 = 0, c1 = 0;
-        if (TILES == 1) {                // columns 0 .. 3 hi, 4 .. 7 lo
-          const bool low = c >= 2;
-          b0 = transpose_8x8(pack_half2(low ? lo[0] : w[0], low ? lo[1] : w[1]));
-          b1 = transpose_8x8(pack_half2(low ? lo[2] : w[2], low ? lo[3] : w[3]));
-        } else {
-          b0 = transpose_8x8(pack_half2(w[0], w[1]));
-          b1 = transpose_8x8(pack_half2(w[2], w[3]));
-          c0 = transpose_8x8(pack_half2(lo[0], lo[1]));
-          c1 = transpose_8x8(pack_half2(lo[2], lo[3]));
-        }
-        #pragma unroll
-        for (int i = 0; i < KSTEPS; ++i) {
-          // rows g and g + 8 of tile i: bytes 2i and 2i + 1 of this lane's piece; pairs of keys (0, 1) and (2, 3)
-          const uint32_t sel = i & 1 ? 0x7362u : 0x5140u;
-          const uint32_t x = __byte_perm(vw[t][0][i / 2], vw[t][1][i / 2], sel);
-          const uint32_t y = __byte_perm(vw[t][2][i / 2], vw[t][3][i / 2], sel);
-          const uint32_t a0 = half2_of_e4m3x2(x & 0xffffu), a1 = half2_of_e4m3x2(x >> 16);
-          const uint32_t a2 = half2_of_e4m3x2(y & 0xffffu), a3 = half2_of_e4m3x2(y >> 16);
-          mma_16816(part[0][i], a0, a1, a2, a3, b0, b1);
-          if (TILES == 2) mma_16816(part[TILES - 1][i], a0, a1, a2, a3, c0, c1);
-        }
+      for (int j = 0; j < KSTEPS; ++j) {
+        uint32_t a0, a1, a2, a3;
+        widen(k0[j], a0, a2);
+        widen(k1[j], a1, a3);
+        mma_16816(d, a0, a1, a2, a3, qf[j][0], qf[j][1]);
       }
       #pragma unroll
-      for (int t = 0; t < TILES; ++t)
-        #pragma unroll
-        for (int i = 0; i < KSTEPS; ++i)
-          #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[t][i][e] = fmaf(part[t][i][e], v_scale, acc[t][i][e] * alpha[e & 1]);
+      for (int i = 0; i < COLS; ++i) { s[t][i] = d[i]; s[t][COLS + i] = d[2 + i]; }
     }
+    float f[COLS];
+    #pragma unroll
+    for (int i = 0; i < COLS; ++i) f[i] = col_scale[i] * k_scale;
+    // ---- bias: one value beyond the largest distance on either side, a small table within it
+    float far_bias = 0.f;
+    bool near = false;
+    if (has_bias) {
+      const bool before = n0 + ITEM - 1 - first_pos <= -md, after = n0 - last_pos >= md;
+      near = !before && !after;
+      if (near) {
+        // entry i: key n0 + i - (ROWS - 1) and the first row
+        __syncwarp();
+        #pragma unroll 1
+        for (int i = 0; i < NEAR - 1; i += 32) {
+          const float v = bias_of(n0 + i + lane - (ROWS - 1) - first_pos);
+          if (i + lane < NEAR - 1) near_bias[warp][i + lane] = v;
+        }
+        __syncwarp();
+      } else {
+        far_bias = before ? bias_before : bias_after;
+      }
+    }
+    float mx[COLS];
+    #pragma unroll
+    for (int i = 0; i < COLS; ++i) mx[i] = -INFINITY;
+    #pragma unroll
+    for (int t = 0; t < SUB; ++t)
+      #pragma unroll
+      for (int e = 0; e < 2 * COLS; ++e) {
+        const int i = e % COLS, key = t * 16 + key_of_g + 8 * (e / COLS);
+        float bias = far_bias;
+        if (near) bias = near_bias[warp][key + ROWS - 1 - (col_pos[i] - first_pos)];
+        s[t][e] = fmaf(s[t][e], f[i], bias);
+        if (!whole && (n0 + key >= n_end || (p.causal && n0 + key > col_pos[i]))) s[t][e] = -INFINITY;
+        mx[i] = fmaxf(mx[i], s[t][e]);
+      }
+    // ---- running maximum, weights
+    float alpha[COLS], ref[COLS];
+    #pragma unroll
+    for (int i = 0; i < COLS; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 4));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 8));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 16));
+      const float m_new = fmaxf(m_run[i], mx[i]);
+      ref[i] = m_new == -INFINITY ? 0.f : m_new;
+      alpha[i] = fast_exp2(m_run[i] - ref[i]);
+      m_run[i] = m_new;
+      l_run[i] *= alpha[i];
+    }
+    float part[TILES][KSTEPS][4];
+    #pragma unroll
+    for (int t = 0; t < TILES; ++t)
+      #pragma unroll
+      for (int i = 0; i < KSTEPS; ++i)
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) part[t][i][e] = 0.f;
+    #pragma unroll
+    for (int t = 0; t < SUB; ++t) {
+      float w[2 * COLS], hi[2 * COLS], lo[2 * COLS];
+      #pragma unroll
+      for (int e = 0; e < 2 * COLS; ++e) {
+        w[e] = fast_exp2(s[t][e] - ref[e % COLS]);
+        l_run[e % COLS] += w[e];
+        hi[e] = __uint_as_float(__float_as_uint(w[e]) & 0xffffe000u);
+        lo[e] = w[e] - hi[e];
+      }
+      uint32_t b0, b1, c0 = 0, c1 = 0;
+      if constexpr (TILES == 1) {        // columns 2c and 2c + 1: hi and lo
+        b0 = transpose_8x8(pack_half2(hi[0], lo[0]));
+        b1 = transpose_8x8(pack_half2(hi[1], lo[1]));
+      } else {
+        b0 = transpose_8x8(pack_half2(hi[0], hi[1]));
+        b1 = transpose_8x8(pack_half2(hi[2], hi[3]));
+        c0 = transpose_8x8(pack_half2(lo[0], lo[1]));
+        c1 = transpose_8x8(pack_half2(lo[2], lo[3]));
+      }
+      uint32_t v0[VW], v1[VW], v2[VW], v3[VW];
+      const uint8_t* at = values + (t * 16 + c) * D + VB * g;
+      read_bytes<VB>(at, v0); read_bytes<VB>(at + 4 * D, v1); read_bytes<VB>(at + 8 * D, v2); read_bytes<VB>(at + 12 * D, v3);
+      #pragma unroll
+      for (int i = 0; i < KSTEPS; ++i) {
+        // rows g and g + 8 of tile i: bytes 2i and 2i + 1 of this lane's piece; pairs of keys (0, 1) and (2, 3)
+        const uint32_t sel = i & 1 ? 0x7362u : 0x5140u;
+        uint32_t a0, a1, a2, a3;
+        widen(__byte_perm(v0[i / 2], v1[i / 2], sel), a0, a1);
+        widen(__byte_perm(v2[i / 2], v3[i / 2], sel), a2, a3);
+        mma_16816(part[0][i], a0, a1, a2, a3, b0, b1);
+        if constexpr (TILES == 2) mma_16816(part[1][i], a0, a1, a2, a3, c0, c1);
+      }
+    }
+    #pragma unroll
+    for (int t = 0; t < TILES; ++t)
+      #pragma unroll
+      for (int i = 0; i < KSTEPS; ++i)
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][i][e] = fmaf(part[t][i][e], v_scale, acc[t][i][e] * alpha[TILES == 1 ? 0 : e & 1]);
   }
+  copy_wait<0>();
+  __syncwarp();                          // the ring is free for the warp's result
+  float* sm_o = (float*)ring;            // [ROWS][D]
 
-  // ---- the warp's result: hi + lo, sums over the lanes that share a column
+  // ---- the warp's result: hi + lo, sums over the lanes that share a row
   #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < COLS; ++i) {
     l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 4);
     l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 8);
     l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 16);
-    if (g == 0) { sm_m[warp][2 * c + i] = m_run[i]; sm_l[warp][2 * c + i] = l_run[i]; }
+    if (g == 0) { sm_m[warp][COLS * c + i] = m_run[i]; sm_l[warp][COLS * c + i] = l_run[i]; }
   }
   #pragma unroll
   for (int i = 0; i < KSTEPS; ++i)
     #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float o = acc[0][i][e];
-      if (TILES == 1) o += __shfl_xor_sync(0xffffffffu, o, 2);          // column + 4
-      else o += acc[TILES - 1][i][e];
-      const int row = 2 * c + (e & 1);
-      if (row < ROWS) sm_o[warp][row][VB * g + 2 * i + (e >> 1)] = o;
+    for (int e = 0; e < 2; ++e) {        // bytes 2i and 2i + 1
+      if constexpr (TILES == 1) {
+        sm_o[c * D + VB * g + 2 * i + e] = acc[0][i][2 * e] + acc[0][i][2 * e + 1];
+      } else {
+        sm_o[2 * c * D + VB * g + 2 * i + e] = acc[0][i][2 * e] + acc[1][i][2 * e];
+        sm_o[(2 * c + 1) * D + VB * g + 2 * i + e] = acc[0][i][2 * e + 1] + acc[1][i][2 * e + 1];
+      }
     }
   __syncthreads();
 
@@ -320,7 +436,7 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
     for (int w = 0; w < WARPS; ++w) {
       const float f = fast_exp2(sm_m[w][r] - ref);
       l += sm_l[w][r] * f;
-      o += sm_o[w][r][d] * f;
+      o += ((const float*)(rings + w * R::WARP_BYTES))[r * D + d] * f;
     }
     if (C == 1) {
       if (m0 + r < p.M)
@@ -351,41 +467,65 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
   cluster.sync();                        // nobody leaves while its shared memory is read
 }
 
-static int cluster_blocks(int64_t heads, int N) {
-  // as many blocks per head as fill the GPU a few times over, each with at least a block of 64 keys per warp
-  const int64_t most = (N + WARPS * BLOCK - 1) / (WARPS * BLOCK);
-  int C = 1;
-  while (C < MAX_CLUSTER && heads * C < 8 * 148 && C * 2 <= most) C *= 2;
-  return C;
-}
-
-template <typename T, int D, int TILES>
-static int launch(const Params& p, const BucketSpec& spec, size_t smem, cudaStream_t stream) {
-  const int C = cluster_blocks((int64_t)p.B * p.H * p.row_groups, p.N);
+template <typename T, int D, int TILES, int WARPS>
+static int launch(const Params& p, const BucketSpec& spec, int C, cudaStream_t stream) {
+  constexpr int smem = WARPS * Ring<D>::WARP_BYTES;
+  static std::atomic<bool> ready[64];    // per device: more shared memory, clusters of 16 (setting them twice is harmless)
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return T5B_ERR_LAUNCH;
+  if (!ready[dev]) {
+    const auto kernel = decode_quantized_kernel<T, D, TILES, WARPS>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return T5B_ERR_LAUNCH;
+    ready[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)C, (unsigned)p.H, (unsigned)(p.B * p.row_groups));
-  cfg.blockDim = dim3(THREADS); cfg.stream = stream; cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(WARPS * 32); cfg.stream = stream; cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)C; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, decode_quantized_kernel<T, D, TILES>, p, spec) == cudaSuccess ? T5B_OK : T5B_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, decode_quantized_kernel<T, D, TILES, WARPS>, p, spec) == cudaSuccess ? T5B_OK : T5B_ERR_LAUNCH;
+}
+
+// Warps per head: few heads get as many as keep the GPU full at once (20 a multiprocessor), one item each at least; with
+// more heads than that, blocks of four warps in clusters such that a warp still has eight items, so that the last
+// blocks are a small part of the whole.
+#ifndef DQ_ROOM
+#define DQ_ROOM 20
+#endif
+#ifndef DQ_RULE
+#define DQ_RULE 8
+#endif
+template <typename T, int D, int TILES>
+static int launch_split(const Params& p, const BucketSpec& spec, cudaStream_t stream) {
+  const int64_t heads = (int64_t)p.B * p.H * p.row_groups, items = (p.N + 31) / 32;
+  const int64_t room = DQ_ROOM * 148 / heads;
+  if (room >= 8 && items > 4) {
+    int C = 1;
+    while (C < MAX_CLUSTER && 16 * C <= room && 16 * C < items) C *= 2;
+    return launch<T, D, TILES, 8>(p, spec, C, stream);
+  }
+  int C = 1;
+  while (C < 8 && items >= 4 * 2 * C * DQ_RULE) C *= 2;
+  return launch<T, D, TILES, 4>(p, spec, C, stream);
 }
 
 template <typename T, int D>
-static int launch_rows(Params& p, const BucketSpec& spec, size_t smem, cudaStream_t stream) {
+static int launch_rows(Params& p, const BucketSpec& spec, cudaStream_t stream) {
   p.row_groups = p.M <= 4 ? 1 : (p.M + 7) / 8;
   if ((int64_t)p.B * p.row_groups > 65535) return T5B_ERR_SHAPE;
-  return p.M <= 4 ? launch<T, D, 1>(p, spec, smem, stream) : launch<T, D, 2>(p, spec, smem, stream);
+  return p.M <= 4 ? launch_split<T, D, 1>(p, spec, stream) : launch_split<T, D, 2>(p, spec, stream);
 }
 
 template <typename T>
-static int launch_type(Params& p, int D, const BucketSpec& spec, size_t smem, cudaStream_t stream) {
+static int launch_type(Params& p, int D, const BucketSpec& spec, cudaStream_t stream) {
   switch (D) {
-    case 16: return launch_rows<T, 16>(p, spec, smem, stream);
-    case 32: return launch_rows<T, 32>(p, spec, smem, stream);
-    case 64: return launch_rows<T, 64>(p, spec, smem, stream);
-    case 128: return launch_rows<T, 128>(p, spec, smem, stream);
+    case 16: return launch_rows<T, 16>(p, spec, stream);
+    case 32: return launch_rows<T, 32>(p, spec, stream);
+    case 64: return launch_rows<T, 64>(p, spec, stream);
+    case 128: return launch_rows<T, 128>(p, spec, stream);
   }
   return T5B_ERR_HEAD_DIM;
 }
@@ -424,8 +564,8 @@ extern "C" int t5b_decode_quantized_fwd(const t5b_decode_quantized_args* a, void
   p.table_stride0 = a->table_stride0; p.table_dtype = a->table_dtype;
   p.B = a->B; p.H = a->H; p.M = a->M; p.N = a->N; p.causal = a->causal; p.q_pos_offset = a->q_pos_offset; p.row_groups = 1;
   p.scale_log2 = a->sm_scale * kLog2e;
-  const size_t smem = a->table ? (size_t)(2 * spec.max_distance + 1) * 4 : 0;
+  p.q_aligned = (uintptr_t)a->q % 8 == 0 && a->q_stride_b % 4 == 0 && a->q_stride_h % 4 == 0 && a->q_stride_m % 4 == 0;
   cudaStream_t st = (cudaStream_t)stream;
-  if (a->dtype == T5B_F16) return decq::launch_type<__half>(p, a->D, spec, smem, st);
-  return decq::launch_type<__nv_bfloat16>(p, a->D, spec, smem, st);
+  if (a->dtype == T5B_F16) return decq::launch_type<__half>(p, a->D, spec, st);
+  return decq::launch_type<__nv_bfloat16>(p, a->D, spec, st);
 }
