@@ -39,20 +39,10 @@ namespace decq {
 
 constexpr int BLOCK = T5B_CACHE_BLOCK;
 constexpr int MAX_CLUSTER = 16;          // more than 8 is beyond what every GPU has to offer, but not this one
-#ifndef DQ_SUB
-#define DQ_SUB 2
-#endif
-#ifndef DQ_STAGES
-#define DQ_STAGES 3
-#endif
-#ifndef DQ_MINW
-#define DQ_MINW 16
-#endif
-
 // 16-key tiles of an item, and how its stages lie in shared memory: keys, values, two scales
 template <int D> struct Ring {
-  static constexpr int SUB = D == 128 ? 2 : D == 64 ? DQ_SUB : 4;
-  static constexpr int STAGES = D == 128 ? 2 : DQ_STAGES;
+  static constexpr int SUB = D == 128 ? 2 : D == 64 ? 2 : 4;
+  static constexpr int STAGES = D == 128 ? 2 : 3;
   static constexpr int ITEM = SUB * 16;
   static constexpr int BYTES = 2 * ITEM * D + 16;
   static constexpr int WARP_BYTES = STAGES * BYTES;
@@ -124,7 +114,7 @@ template <int D> __device__ __forceinline__ int dim_of(int c, int j, int e) {
 // TILES 1: up to four rows, each with two columns of the products (hi and lo of its weights).  TILES 2: up to eight rows,
 // a column each, the second product twice.
 template <typename T, int D, int TILES, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, TILES == 1 && D <= 64 ? DQ_MINW / WARPS : 1)
+__global__ void __launch_bounds__(WARPS * 32, TILES == 1 && D <= 64 ? 16 / WARPS : 1)
 decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant__ BucketSpec spec) {
   using R = Ring<D>;
   constexpr int THREADS = WARPS * 32;
@@ -489,27 +479,23 @@ static int launch(const Params& p, const BucketSpec& spec, int C, cudaStream_t s
   return cudaLaunchKernelEx(&cfg, decode_quantized_kernel<T, D, TILES, WARPS>, p, spec) == cudaSuccess ? T5B_OK : T5B_ERR_LAUNCH;
 }
 
-// Warps per head: few heads get as many as keep the GPU full at once (20 a multiprocessor), one item each at least; with
-// more heads than that, blocks of four warps in clusters such that a warp still has eight items, so that the last
-// blocks are a small part of the whole.
-#ifndef DQ_ROOM
-#define DQ_ROOM 20
-#endif
-#ifndef DQ_RULE
-#define DQ_RULE 8
-#endif
+// Warps per head.  What a block costs beyond its keys (lengths, queries, bias, two merges) and how the last blocks fill the
+// GPU decide, so the split goes by heads = B * H * groups of rows and by the items of a whole cache (us on B200):
+//   * up to 212 heads: a block of eight warps each, and clusters up to 1700 warps in all as long as a warp keeps four items
+//     (192 heads x 2048 keys: 9.4, with four warps 10.3; 12 x 102400: 36.1 in clusters of 16, 267 without);
+//   * short caches of many heads: two warps (768 x 512: 12.8, with four 14.3);
+//   * else four warps (1536 x 2048: 66.9, with two 78.8), two blocks per head for long caches of 400 to 1200 heads, where
+//     one block per head leaves the last round of blocks half empty (1024 x 8192: 165.5, with one 170.2).
 template <typename T, int D, int TILES>
 static int launch_split(const Params& p, const BucketSpec& spec, cudaStream_t stream) {
-  const int64_t heads = (int64_t)p.B * p.H * p.row_groups, items = (p.N + 31) / 32;
-  const int64_t room = DQ_ROOM * 148 / heads;
-  if (room >= 8 && items > 4) {
+  const int64_t heads = (int64_t)p.B * p.H * p.row_groups, items = (p.N + Ring<D>::ITEM - 1) / Ring<D>::ITEM;
+  if (heads <= 212 && items >= 16) {
     int C = 1;
-    while (C < MAX_CLUSTER && 16 * C <= room && 16 * C < items) C *= 2;
+    while (C < MAX_CLUSTER && heads * 16 * C <= 1700 && items >= 64 * C) C *= 2;
     return launch<T, D, TILES, 8>(p, spec, C, stream);
   }
-  int C = 1;
-  while (C < 8 && items >= 4 * 2 * C * DQ_RULE) C *= 2;
-  return launch<T, D, TILES, 4>(p, spec, C, stream);
+  if (heads >= 512 && items <= 16) return launch<T, D, TILES, 2>(p, spec, 1, stream);
+  return launch<T, D, TILES, 4>(p, spec, heads > 400 && heads < 1200 && items >= 256 ? 2 : 1, stream);
 }
 
 template <typename T, int D>
