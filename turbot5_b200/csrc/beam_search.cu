@@ -646,82 +646,103 @@ step_kernel(const __grid_constant__ Params p) {
 
 // ---- sentences from the history of tokens and parents -------------------------------------------------------------
 //
-// Walking back from the last token is a chain of dependent reads.  A block per sentence brings a segment of the parents
-// into shared memory and cuts it into pieces: every piece is walked from each of its K possible beams at once, the
-// pieces' results are chained per returned sentence, and the pieces are walked again from the beam that is now known.
+// Walking back from the last token is a chain of dependent reads.  A block per sentence brings a segment of tokens and
+// parents into shared memory (every read in flight at once) and cuts it into pieces: every piece is walked from each of
+// its K possible beams, the pieces' results are chained per returned sentence, and the pieces are walked again from the
+// beam that is now known.  Three short chains instead of one of T reads from memory.
 constexpr int SEGMENT = 1024;            // steps in shared memory at a time
-constexpr int SEQ_THREADS = 256;
+constexpr int SEQ_THREADS = 512;
+constexpr int PIECES = 32;
 
 struct SequenceParams {
   const int32_t* tokens; const int32_t* parents; const float* scores; const float* fin_scores;
   const int32_t* fin_steps; const int32_t* fin_beams; const uint8_t* done;
   int64_t* out; float* out_scores;
-  int32_t T, B, K, R;
+  int32_t T, B, K, R, k_log2;            // 2^k_log2 >= K
   int64_t eos, pad;
   double length;
 };
 
 __global__ void __launch_bounds__(SEQ_THREADS)
 sequences_kernel(const __grid_constant__ SequenceParams p) {
-  extern __shared__ uint8_t raw[];
+  extern __shared__ __align__(16) uint8_t raw[];
   __shared__ int last[MAX_BEAMS], from[MAX_BEAMS], cur[MAX_BEAMS];
   __shared__ bool ended[MAX_BEAMS], none[MAX_BEAMS];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
   const int K = p.K, R = p.R, T = p.T;
   const int seg = min(SEGMENT, T);
-  uint8_t* par = raw;                    // [seg][K]
-  uint8_t* path = par + seg * K;         // [R][seg]
-  uint8_t* jump = path + seg * R;        // [pieces][K], pieces <= 32
+  int32_t* words = (int32_t*)raw;                // [seg][K]
+  uint8_t* par = raw + (size_t)seg * K * 4;      // [seg][K]
+  uint8_t* path = par + seg * K;                 // [R][seg]
+  uint8_t* jump = path + seg * R;                // [PIECES][K]
+  const int x_of = tid & ((1 << p.k_log2) - 1), t_of = tid >> p.k_log2, rows = SEQ_THREADS >> p.k_log2;
 
-  if (tid < 32) {
-    // candidates: lanes [0, K) the pool, [K, 2K) the running beams
-    const int64_t at = (int64_t)b * K;
-    float v = -INFINITY;
-    if (lane < K) v = p.fin_scores[at + lane];
-    else if (lane < 2 * K && !p.done[b]) v = (float)((double)p.scores[at + lane - K] / p.length);
-    if (!(v == v)) v = -INFINITY;
-    int above = 0;
-    for (int j = 0; j < 2 * K; ++j) {
-      const float o = __shfl_sync(0xffffffffu, v, j);
-      above += o > v || (o == v && j < lane);
-    }
-    if (lane < 2 * K && above < R) {
-      const bool e = lane < K;
-      ended[above] = e; none[above] = v == -INFINITY;
-      // an ended sentence's end token stands at its step, its beams are those up to the step before
-      last[above] = e ? min(max(p.fin_steps[at + lane], 0), T - 1) : T - 1;
-      from[above] = e ? min(max(p.fin_beams[at + lane], 0), K - 1) : lane - K;
-      p.out_scores[(int64_t)b * R + above] = v;
-    }
-  }
-  __syncthreads();
-  if (tid < R) cur[tid] = 0;
   for (int hi = T; hi > 0; hi -= seg) {
     const int lo = max(0, hi - seg), len = hi - lo;
     // par[i]: the beam at step lo + i - 1 of each beam at step lo + i
-    for (int i = tid; i < len * K; i += SEQ_THREADS) {
-      const int t = lo + i / K, x = i % K;
-      par[i] = (uint8_t)min(max(p.parents[((int64_t)t * p.B + b) * K + x], 0), K - 1);
+    #pragma unroll 1
+    for (int t0 = 0; t0 < len; t0 += 8 * rows) {
+      int w[8], q[8];
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int t = t0 + i * rows + t_of;
+        const int64_t at = ((int64_t)(lo + t) * p.B + b) * K + x_of;
+        const bool in = t < len && x_of < K;
+        w[i] = in ? __ldg(p.tokens + at) : 0;
+        q[i] = in ? __ldg(p.parents + at) : 0;
+      }
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int t = t0 + i * rows + t_of;
+        if (t < len && x_of < K) { words[t * K + x_of] = w[i]; par[t * K + x_of] = (uint8_t)min(max(q[i], 0), K - 1); }
+      }
+    }
+    if (hi == T && tid < 32) {
+      // the returned sentences, while the segment is on its way: lanes [0, K) the pool, [K, 2K) the running beams
+      const int64_t at = (int64_t)b * K;
+      float v = -INFINITY;
+      if (lane < K) v = p.fin_scores[at + lane];
+      else if (lane < 2 * K && !p.done[b]) v = (float)((double)p.scores[at + lane - K] / p.length);
+      if (!(v == v)) v = -INFINITY;
+      int above = 0;
+      #pragma unroll 4
+      for (int j = 0; j < 2 * K; ++j) {
+        const float o = __shfl_sync(0xffffffffu, v, j);
+        above += o > v || (o == v && j < lane);
+      }
+      if (lane < 2 * K && above < R) {
+        const bool e = lane < K;
+        ended[above] = e; none[above] = v == -INFINITY;
+        // an ended sentence's end token stands at its step, its beams are those up to the step before
+        last[above] = e ? min(max(p.fin_steps[at + lane], 0), T - 1) : T - 1;
+        from[above] = e ? min(max(p.fin_beams[at + lane], 0), K - 1) : lane - K;
+        cur[above] = 0;
+        p.out_scores[(int64_t)b * R + above] = v;
+      }
     }
     __syncthreads();
-    const int piece = (len + 31) / 32, pieces = (len + piece - 1) / piece;
-    for (int i = tid; i < pieces * K; i += SEQ_THREADS) {
-      const int c = i / K;
-      int x = i % K;
-      for (int j = min((c + 1) * piece, len) - 1; j >= c * piece; --j) x = par[j * K + x];
-      jump[i] = (uint8_t)x;
-    }
+    const int piece = (len + PIECES - 1) / PIECES, pieces = (len + piece - 1) / piece;
+    if (x_of < K)
+      #pragma unroll 1
+      for (int c = t_of; c < pieces; c += rows) {
+        int x = x_of;
+        #pragma unroll 1
+        for (int j = min((c + 1) * piece, len) - 1; j >= c * piece; --j) x = par[j * K + x];
+        jump[c * K + x_of] = (uint8_t)x;
+      }
     __syncthreads();
     // entry beam of every piece per sentence (kept in path's last step of the piece), backwards
     if (tid < R) {
       const int stop = ended[tid] ? last[tid] - 1 : last[tid];
       int x = cur[tid];
+      #pragma unroll 1
       for (int c = pieces - 1; c >= 0; --c) {
         const int a = c * piece, z = min(a + piece, len) - 1;
         path[tid * seg + z] = (uint8_t)x;
         if (lo + a > stop) continue;                     // the sentence ends before this piece
         if (lo + z >= stop) {                            // ... inside it: walked step by step
           x = from[tid];
+          #pragma unroll 1
           for (int j = stop - lo; j >= a; --j) x = par[j * K + x];
         } else {
           x = jump[c * K + x];
@@ -730,22 +751,23 @@ sequences_kernel(const __grid_constant__ SequenceParams p) {
       cur[tid] = x;
     }
     __syncthreads();
-    for (int i = tid; i < R * pieces; i += SEQ_THREADS) {
-      const int r = i / pieces, c = i % pieces, a = c * piece, z = min(a + piece, len) - 1;
+    for (int r = tid / PIECES; r < R; r += SEQ_THREADS / PIECES) {
+      const int c = tid % PIECES, a = c * piece, z = min(a + piece, len) - 1;
+      if (c >= pieces) continue;
       const int stop = ended[r] ? last[r] - 1 : last[r];
       int x = path[r * seg + z], j = z;
       if (lo + z >= stop) { j = min(z, stop - lo); x = from[r]; }
+      #pragma unroll 1
       for (; j >= a; --j) { path[r * seg + j] = (uint8_t)x; x = par[j * K + x]; }
     }
     __syncthreads();
-    for (int i = tid; i < R * len; i += SEQ_THREADS) {
-      const int r = i / len, t = lo + i % len;
-      int64_t word = p.pad;
-      if (!none[r]) {
-        if (ended[r] && t == last[r]) word = p.eos;
-        else if (t <= last[r]) word = p.tokens[((int64_t)t * p.B + b) * K + path[r * seg + t - lo]];
+    #pragma unroll 1
+    for (int r = 0; r < R; ++r) {
+      const int stop = none[r] ? -1 : ended[r] ? last[r] - 1 : last[r], end = ended[r] && !none[r] ? last[r] : -1;
+      for (int i = tid; i < len; i += SEQ_THREADS) {
+        const int t = lo + i;
+        p.out[((int64_t)b * R + r) * T + t] = t <= stop ? (int64_t)words[i * K + path[r * seg + i]] : t == end ? p.eos : p.pad;
       }
-      p.out[((int64_t)b * R + r) * T + t] = word;
     }
     __syncthreads();
   }
@@ -834,8 +856,13 @@ extern "C" int t5b_beam_search_sequences(const t5b_beam_sequences_args* a, void*
   p.T = a->steps; p.B = a->B; p.K = a->num_beams; p.R = a->num_return;
   p.eos = a->eos_token_id; p.pad = a->pad_token_id;
   p.length = pow((double)a->steps, a->length_penalty);
+  for (p.k_log2 = 0; 1 << p.k_log2 < p.K;) ++p.k_log2;
   const int seg = a->steps < beam::SEGMENT ? a->steps : beam::SEGMENT;
-  const size_t smem = (size_t)seg * (p.K + p.R) + 32 * p.K;
+  const size_t smem = (size_t)seg * (5 * p.K + p.R) + beam::PIECES * p.K;
+  if (smem > 32 * 1024) {
+    constexpr int most = beam::SEGMENT * 6 * beam::MAX_BEAMS + beam::PIECES * beam::MAX_BEAMS;
+    if (cudaFuncSetAttribute(beam::sequences_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) return T5B_ERR_LAUNCH;
+  }
   beam::sequences_kernel<<<(unsigned)p.B, beam::SEQ_THREADS, smem, (cudaStream_t)stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? T5B_OK : T5B_ERR_LAUNCH;
 }
