@@ -668,15 +668,26 @@ sequences_kernel(const __grid_constant__ SequenceParams p) {
   extern __shared__ __align__(16) uint8_t raw[];
   __shared__ int last[MAX_BEAMS], from[MAX_BEAMS], cur[MAX_BEAMS];
   __shared__ bool ended[MAX_BEAMS], none[MAX_BEAMS];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
-  const int K = p.K, R = p.R, T = p.T;
-  const int seg = min(SEGMENT, T);
-  int32_t* words = (int32_t*)raw;                // [seg][K]
-  uint8_t* par = raw + (size_t)seg * K * 4;      // [seg][K]
-  uint8_t* path = par + seg * K;                 // [R][seg]
-  uint8_t* jump = path + seg * R;                // [PIECES][K]
-  const int x_of = tid & ((1 << p.k_log2) - 1), t_of = tid >> p.k_log2, rows = SEQ_THREADS >> p.k_log2;
+  __shared__ int2 cut[MAX_BEAMS];                          // last step with a token of its own, and the end token's
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int K = p.K, R = p.R, T = p.T, kl = p.k_log2;
+  const int seg = min(SEGMENT, T), pitch = (seg + 31) / 32 * 32 + 4;       // (no bank conflicts by step or by beam)
+  int32_t* words = (int32_t*)raw;                          // [K][pitch]
+  uint8_t* par = raw + (size_t)K * pitch * 4;              // [seg][2^kl]
+  uint8_t* path = par + ((size_t)seg << kl);               // [R][pitch]
+  uint8_t* jump = path + (size_t)R * pitch;                // [PIECES][2^kl]
+  const int x_of = tid & ((1 << kl) - 1), t_of = tid >> kl, rows = SEQ_THREADS >> kl;
 
+  // the candidates: lanes [0, K) of the first warp the pool, [K, 2K) the running beams
+  float value = -INFINITY;
+  int their_step = 0, their_beam = 0;
+  bool finished = false;
+  if (warp == 0) {
+    const int64_t at = (int64_t)b * K;
+    finished = p.done[b];
+    if (lane < K) { value = p.fin_scores[at + lane]; their_step = p.fin_steps[at + lane]; their_beam = p.fin_beams[at + lane]; }
+    else if (lane < 2 * K) value = p.scores[at + lane - K];
+  }
   for (int hi = T; hi > 0; hi -= seg) {
     const int lo = max(0, hi - seg), len = hi - lo;
     // par[i]: the beam at step lo + i - 1 of each beam at step lo + i
@@ -694,79 +705,87 @@ sequences_kernel(const __grid_constant__ SequenceParams p) {
       #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int t = t0 + i * rows + t_of;
-        if (t < len && x_of < K) { words[t * K + x_of] = w[i]; par[t * K + x_of] = (uint8_t)min(max(q[i], 0), K - 1); }
+        if (t < len && x_of < K) { words[x_of * pitch + t] = w[i]; par[t << kl | x_of] = (uint8_t)min(max(q[i], 0), K - 1); }
       }
     }
-    if (hi == T && tid < 32) {
-      // the returned sentences, while the segment is on its way: lanes [0, K) the pool, [K, 2K) the running beams
-      const int64_t at = (int64_t)b * K;
-      float v = -INFINITY;
-      if (lane < K) v = p.fin_scores[at + lane];
-      else if (lane < 2 * K && !p.done[b]) v = (float)((double)p.scores[at + lane - K] / p.length);
-      if (!(v == v)) v = -INFINITY;
+    if (hi == T && warp == 0) {
+      // the best of them, best first
+      if (lane >= K) value = finished || lane >= 2 * K ? -INFINITY : (float)((double)value / p.length);
+      if (!(value == value)) value = -INFINITY;
       int above = 0;
       #pragma unroll 4
       for (int j = 0; j < 2 * K; ++j) {
-        const float o = __shfl_sync(0xffffffffu, v, j);
-        above += o > v || (o == v && j < lane);
+        const float o = __shfl_sync(0xffffffffu, value, j);
+        above += o > value || (o == value && j < lane);
       }
       if (lane < 2 * K && above < R) {
         const bool e = lane < K;
-        ended[above] = e; none[above] = v == -INFINITY;
+        ended[above] = e; none[above] = value == -INFINITY;
         // an ended sentence's end token stands at its step, its beams are those up to the step before
-        last[above] = e ? min(max(p.fin_steps[at + lane], 0), T - 1) : T - 1;
-        from[above] = e ? min(max(p.fin_beams[at + lane], 0), K - 1) : lane - K;
+        last[above] = e ? min(max(their_step, 0), T - 1) : T - 1;
+        from[above] = e ? min(max(their_beam, 0), K - 1) : lane - K;
         cur[above] = 0;
-        p.out_scores[(int64_t)b * R + above] = v;
+        p.out_scores[(int64_t)b * R + above] = value;
       }
     }
     __syncthreads();
-    const int piece = (len + PIECES - 1) / PIECES, pieces = (len + piece - 1) / piece;
+    int pl = 0;                                            // pieces of 2^pl steps, at most PIECES of them
+    while (2 << 2 * pl < len) ++pl;
+    const int pieces = (len + (1 << pl) - 1) >> pl;
     if (x_of < K)
       #pragma unroll 1
       for (int c = t_of; c < pieces; c += rows) {
         int x = x_of;
-        #pragma unroll 1
-        for (int j = min((c + 1) * piece, len) - 1; j >= c * piece; --j) x = par[j * K + x];
-        jump[c * K + x_of] = (uint8_t)x;
+        const uint8_t* at = par + ((min((c + 1) << pl, len) - 1) << kl);
+        #pragma unroll 4
+        for (int j = min((c + 1) << pl, len) - (c << pl); j > 0; --j, at -= 1 << kl) x = at[x];
+        jump[c << kl | x_of] = (uint8_t)x;
       }
     __syncthreads();
-    // entry beam of every piece per sentence (kept in path's last step of the piece), backwards
+    // the beam at the last step of every piece per sentence, backwards; kept there in path
     if (tid < R) {
-      const int stop = ended[tid] ? last[tid] - 1 : last[tid];
-      int x = cur[tid];
+      const int stop = (ended[tid] ? last[tid] - 1 : last[tid]) - lo;                  // its last step, in this segment's
+      int x = cur[tid], c = pieces - 1;
+      if (stop >= 0 && stop < len) {                       // ... which is in here: its piece is walked step by step
+        c = stop >> pl;
+        x = from[tid];
+        path[tid * pitch + stop] = (uint8_t)x;
+        for (int j = stop; j >= c << pl; --j) x = par[j << kl | x];
+        --c;
+      } else if (stop < 0) {
+        c = -1;
+      }
+      uint8_t* at = path + tid * pitch;
       #pragma unroll 1
-      for (int c = pieces - 1; c >= 0; --c) {
-        const int a = c * piece, z = min(a + piece, len) - 1;
-        path[tid * seg + z] = (uint8_t)x;
-        if (lo + a > stop) continue;                     // the sentence ends before this piece
-        if (lo + z >= stop) {                            // ... inside it: walked step by step
-          x = from[tid];
-          #pragma unroll 1
-          for (int j = stop - lo; j >= a; --j) x = par[j * K + x];
-        } else {
-          x = jump[c * K + x];
-        }
+      for (; c >= 0; --c) {
+        at[min((c + 1) << pl, len) - 1] = (uint8_t)x;
+        x = jump[c << kl | x];
       }
       cur[tid] = x;
     }
     __syncthreads();
-    for (int r = tid / PIECES; r < R; r += SEQ_THREADS / PIECES) {
-      const int c = tid % PIECES, a = c * piece, z = min(a + piece, len) - 1;
-      if (c >= pieces) continue;
-      const int stop = ended[r] ? last[r] - 1 : last[r];
-      int x = path[r * seg + z], j = z;
-      if (lo + z >= stop) { j = min(z, stop - lo); x = from[r]; }
+    for (int r = warp; r < R; r += SEQ_THREADS / 32) {
+      const int a = lane << pl, stop = (ended[r] ? last[r] - 1 : last[r]) - lo;
+      int j = min(min(a + (1 << pl), len) - 1, stop);
+      if (lane >= pieces || j < a) continue;
+      int x = path[r * pitch + j];
       #pragma unroll 1
-      for (; j >= a; --j) { path[r * seg + j] = (uint8_t)x; x = par[j * K + x]; }
+      for (; j > a; --j) { x = par[j << kl | x]; path[r * pitch + j - 1] = (uint8_t)x; }
     }
     __syncthreads();
+    // a thread has a step of every sentence
     #pragma unroll 1
-    for (int r = 0; r < R; ++r) {
-      const int stop = none[r] ? -1 : ended[r] ? last[r] - 1 : last[r], end = ended[r] && !none[r] ? last[r] : -1;
-      for (int i = tid; i < len; i += SEQ_THREADS) {
-        const int t = lo + i;
-        p.out[((int64_t)b * R + r) * T + t] = t <= stop ? (int64_t)words[i * K + path[r * seg + i]] : t == end ? p.eos : p.pad;
+    for (int r = warp; r < R; r += SEQ_THREADS / 32) cut[r] = make_int2((none[r] ? -1 : ended[r] ? last[r] - 1 : last[r]) - lo,
+                                                                        (ended[r] && !none[r] ? last[r] : -1) - lo);
+    __syncthreads();
+    for (int i = tid; i < len; i += SEQ_THREADS) {
+      int64_t* out = p.out + (int64_t)b * R * T + lo + i;
+      #pragma unroll 4
+      for (int r = 0; r < R; ++r, out += T) {
+        const int2 at = cut[r];
+        const int beam = i <= at.x ? path[r * pitch + i] : 0;
+        const int word = words[beam * pitch + i];
+        *out = i <= at.x ? (int64_t)word : i == at.y ? p.eos : p.pad;
       }
     }
     __syncthreads();
@@ -857,10 +876,10 @@ extern "C" int t5b_beam_search_sequences(const t5b_beam_sequences_args* a, void*
   p.eos = a->eos_token_id; p.pad = a->pad_token_id;
   p.length = pow((double)a->steps, a->length_penalty);
   for (p.k_log2 = 0; 1 << p.k_log2 < p.K;) ++p.k_log2;
-  const int seg = a->steps < beam::SEGMENT ? a->steps : beam::SEGMENT;
-  const size_t smem = (size_t)seg * (5 * p.K + p.R) + beam::PIECES * p.K;
+  const int seg = a->steps < beam::SEGMENT ? a->steps : beam::SEGMENT, pitch = (seg + 31) / 32 * 32 + 4;
+  const size_t smem = (size_t)p.K * pitch * 4 + ((size_t)(seg + beam::PIECES) << p.k_log2) + (size_t)p.R * pitch;
   if (smem > 32 * 1024) {
-    constexpr int most = beam::SEGMENT * 6 * beam::MAX_BEAMS + beam::PIECES * beam::MAX_BEAMS;
+    constexpr int most = (beam::SEGMENT + 36) * 6 * beam::MAX_BEAMS;
     if (cudaFuncSetAttribute(beam::sequences_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) return T5B_ERR_LAUNCH;
   }
   beam::sequences_kernel<<<(unsigned)p.B, beam::SEQ_THREADS, smem, (cudaStream_t)stream>>>(p);
