@@ -26,7 +26,9 @@ from torch import nn
 
 from . import _native as nat
 from .attention import (flash_attention_with_fusing_bias, flash_attention_with_fusing_bias_varlen,
-                        flash_decoding_with_fusing_bias)
+                        flash_decoding_quantized_with_fusing_bias, flash_decoding_with_fusing_bias)
+from .generation import (CACHE_BLOCK, MAX_BEAMS, beam_search_sequences, beam_search_step, quantize_into_cache,
+                         reorder_beam_cache)
 from .modules import (T5ATTENTION_TYPES, T5FlashAttention, T5LayerNorm, add_rms_layer_norm, gated_gelu,
                       rms_layer_norm)
 from .padding import get_unpad_plan, pad_rows, unpad_rows
@@ -54,6 +56,8 @@ class T5StackConfig:
     decoder_start_token_id: int = 0
     attention_type: str = "flash"              # encoder self-attention: "flash" (full) or "local" (block-local)
     sliding_window: int = 512                  # block length of the "local" type
+    eos_token_id: int = 1
+    pad_token_id: int = 0
 
 
 class _FusedOps:
@@ -129,16 +133,116 @@ class DecoderCache:
     """Preallocated K/V cache of one generation: self-attention keys/values grow in place,
     cross-attention keys/values are projected once from the encoder output.  Keys and values of a
     layer's self-attention live in ONE tensor (2, B, H, max_len, D), so that a decoding step appends
-    both with one copy; `self_k[i]` / `self_v[i]` are its two halves."""
+    both with one copy; `self_k[i]` / `self_v[i]` are its two halves.
 
-    def __init__(self, n_layers, batch, heads, d_kv, max_len, dtype, device):
-        self.self_kv = [torch.empty((2, batch, heads, max_len, d_kv), dtype=dtype, device=device) for _ in range(n_layers)]
+    With `beams` the self-attention has a row for each of a sentence's beams, while the cross-attention's rows are the
+    sentences: their beams read them together."""
+    scales = ()
+    workspace = None        # split scratch of this cache's own, or the one kept per stream
+
+    def __init__(self, n_layers, batch, heads, d_kv, max_len, dtype, device, beams=1):
+        self.self_kv = [torch.empty((2, batch * beams, heads, max_len, d_kv), dtype=dtype, device=device)
+                        for _ in range(n_layers)]
         self.self_k = [kv[0] for kv in self.self_kv]
         self.self_v = [kv[1] for kv in self.self_kv]
         self.cross_k: List[Optional[torch.Tensor]] = [None] * n_layers
         self.cross_v: List[Optional[torch.Tensor]] = [None] * n_layers
         self.length = 0
         self.max_len = max_len
+        self.beams = beams
+
+    def set_cross(self, i, k, v, seqlens=None):
+        self.cross_k[i], self.cross_v[i] = k, v
+
+    def own_workspace(self):
+        """Scratch for the split-KV launches that no other cache shares: captured graphs of two caches may then run at
+        the same time."""
+        L, (_, rows, H, cap, D) = nat.lib(), self.self_kv[0].shape
+        need = L.t5b_decode_workspace_bytes(rows, H, 1, D, max(1, L.t5b_decode_num_splits(rows, H, cap)))
+        for k in self.cross_k:
+            if k is not None:
+                B, _, N, _ = k.shape
+                need = max(need, L.t5b_decode_workspace_bytes(B, H, self.beams, D, max(1, L.t5b_decode_num_splits(B, H, N))))
+        self.workspace = torch.zeros(max(need, 256), dtype=torch.uint8, device=self.self_kv[0].device)
+
+    def append(self, i, k, v, start):
+        """New keys and values (B, H, M, D) at `start`: a number, or an int64 tensor for a single token."""
+        if torch.is_tensor(start):
+            self.self_k[i].index_copy_(2, start, k)
+            self.self_v[i].index_copy_(2, start, v)
+        else:
+            self.self_k[i][:, :, start:start + k.shape[2]] = k
+            self.self_v[i][:, :, start:start + k.shape[2]] = v
+
+    def append_stacked(self, i, kv, pos):
+        """The single new token's key and value, side by side (B, 1, 2, H, D): one copy."""
+        self.self_kv[i].index_copy_(3, pos, kv.permute(2, 0, 3, 1, 4))
+
+    def attend_self(self, i, q, table, nb, md, kv_len=None, seqlens=None, num_splits=0):
+        return flash_decoding_with_fusing_bias(q, self.self_k[i], self.self_v[i], table, causal=True, sm_scale=1.0,
+                                               NUM_BUCKETS=nb, MAX_DISTANCE=md, kv_len=kv_len, seqlens_k=seqlens,
+                                               num_splits=num_splits, workspace=self.workspace)
+
+    def attend_cross(self, i, q, seqlens=None):
+        return flash_decoding_with_fusing_bias(q, self.cross_k[i], self.cross_v[i], None, causal=False, sm_scale=1.0,
+                                               seqlens_k=seqlens, q_pos_offset=0, workspace=self.workspace)
+
+    def reorder(self, parents, seqlens=None):
+        """Let the self-attention rows follow their beams (`reorder_beam_cache`)."""
+        reorder_beam_cache(self.self_kv, parents, seqlens=seqlens, scales=self.scales)
+
+
+class QuantizedDecoderCache(DecoderCache):
+    """A `DecoderCache` in 8 bits: float8_e4m3fn with a scale per 64 tokens and head, half of the memory and of the
+    bytes that a step reads.  For 16-bit models."""
+
+    def __init__(self, n_layers, batch, heads, d_kv, max_len, dtype, device, beams=1):
+        if dtype not in _HALF:
+            raise ValueError("an 8-bit cache belongs to a float16 or bfloat16 model, got %s" % dtype)
+        if d_kv not in (16, 32, 64, 128):
+            raise ValueError("an 8-bit cache takes head dims 16, 32, 64 and 128, got %d" % d_kv)
+        blocks = -(-max_len // CACHE_BLOCK)
+        super().__init__(n_layers, batch, heads, d_kv, blocks * CACHE_BLOCK, torch.float8_e4m3fn, device, beams)
+        self.max_len = max_len
+        self.scales = [torch.ones((2, batch * beams, heads, blocks), dtype=torch.float32, device=device)
+                       for _ in range(n_layers)]
+        self.cross_scales: List[Optional[torch.Tensor]] = [None] * n_layers
+        self.cross_len = 0
+
+    def set_cross(self, i, k, v, seqlens=None):
+        B, H, N, D = k.shape
+        blocks = max(1, -(-N // CACHE_BLOCK))
+        kv = torch.empty((2, B, H, blocks * CACHE_BLOCK, D), dtype=torch.float8_e4m3fn, device=k.device)
+        scale = torch.ones((2, B, H, blocks), dtype=torch.float32, device=k.device)
+        quantize_into_cache(k, v, kv[0], scale[0], kv[1], scale[1], 0, seqlens=seqlens)
+        self.cross_k[i], self.cross_v[i], self.cross_scales[i], self.cross_len = kv[0], kv[1], scale, N
+
+    def append(self, i, k, v, start):
+        s = self.scales[i]
+        quantize_into_cache(k, v, self.self_k[i], s[0], self.self_v[i], s[1], start)
+
+    def append_stacked(self, i, kv, pos):
+        k, v = kv.transpose(1, 3).unbind(2)              # (B, H, 1, D) each
+        self.append(i, k, v, pos)
+
+    def attend_self(self, i, q, table, nb, md, kv_len=None, seqlens=None, num_splits=0):
+        s = self.scales[i]
+        return flash_decoding_quantized_with_fusing_bias(q, self.self_k[i], s[0], self.self_v[i], s[1], table, causal=True,
+                                                         sm_scale=1.0, NUM_BUCKETS=nb, MAX_DISTANCE=md, kv_len=kv_len,
+                                                         seqlens_k=seqlens)
+
+    def attend_cross(self, i, q, seqlens=None):
+        s = self.cross_scales[i]
+        return flash_decoding_quantized_with_fusing_bias(q, self.cross_k[i], s[0], self.cross_v[i], s[1], None, sm_scale=1.0,
+                                                         kv_len=self.cross_len, seqlens_k=seqlens, q_pos_offset=0)
+
+
+def _cache_class(cache_dtype):
+    if cache_dtype is None:
+        return DecoderCache
+    if cache_dtype == torch.float8_e4m3fn:
+        return QuantizedDecoderCache
+    raise ValueError("cache_dtype is None (the model's type) or torch.float8_e4m3fn, got %s" % cache_dtype)
 
 
 class _NativeState:
@@ -452,16 +556,18 @@ class T5Stack(nn.Module):
         return normed if plan is None else self._unpacked(normed[0], plan, packed_rows, return_packed)
 
     # ---- generation with a preallocated cache (decoder only)
-    def new_cache(self, encoder_hidden_states, max_len) -> DecoderCache:
+    def new_cache(self, encoder_hidden_states, max_len, beams=1, cache_dtype=None, encoder_seqlens=None) -> DecoderCache:
+        """A cache for `max_len` steps over these encoder states, in the model's type or (`cache_dtype`
+        torch.float8_e4m3fn) in 8 bits; `beams` rows of self-attention per sentence.  `encoder_seqlens`: only so many
+        states of each sentence count for the scales of an 8-bit cache."""
         cfg = self.cfg
         B = encoder_hidden_states.shape[0]
-        cache = DecoderCache(len(self.block), B, cfg.num_heads, cfg.d_kv, max_len, encoder_hidden_states.dtype,
-                             encoder_hidden_states.device)
+        cache = _cache_class(cache_dtype)(len(self.block), B, cfg.num_heads, cfg.d_kv, max_len, encoder_hidden_states.dtype,
+                                          encoder_hidden_states.device, beams)
         for i, blk in enumerate(self.block):
             att = blk.layer[1].EncDecAttention
             shape = lambda x: x.view(B, -1, cfg.num_heads, cfg.d_kv).transpose(1, 2)
-            cache.cross_k[i] = shape(att.k(encoder_hidden_states))
-            cache.cross_v[i] = shape(att.v(encoder_hidden_states))
+            cache.set_cross(i, shape(att.k(encoder_hidden_states)), shape(att.v(encoder_hidden_states)), encoder_seqlens)
         return cache
 
     def decode_step_static(self, input_ids, cache: DecoderCache, pos, seqlens, encoder_seqlens=None):
@@ -476,6 +582,9 @@ class T5Stack(nn.Module):
         copy that appends the new key and value to the cache, the split-KV kernel, the output
         projection, residual add + RMSNorm in one kernel -- thirteen launches per layer instead of
         twenty.
+
+        With a cache of several beams, `input_ids` and `seqlens` have a row per beam and `encoder_seqlens` one per
+        sentence.
         """
         cfg = self.cfg
         B = input_ids.shape[0]
@@ -487,6 +596,9 @@ class T5Stack(nn.Module):
         table = self._table()
         fused = hidden.dtype in (torch.bfloat16, torch.float16) and cfg.d_model % 8 == 0
         shape = lambda x: x.view(B, 1, H, D).transpose(1, 2)
+        # cross attention: the beams of a sentence are query rows over its keys
+        K = cache.beams
+        cross = shape if K == 1 else (lambda x: x.view(B // K, K, H, D).transpose(1, 2))
         # The split count of the self-attention launch comes from the cache CAPACITY, not from the
         # current length, so it is the same in every replay (a split beyond the cached keys is empty
         # and merges as such); a small batch then still fills the GPU late in a long generation.
@@ -502,25 +614,20 @@ class T5Stack(nn.Module):
                 w = self._stacked_weights(i)
                 qkv = nn.functional.linear(normed, w["qkv"])                       # (B, 1, 3*H*D)
                 q = shape(qkv[..., :HD])
-                # new key and value -> slot `pos` of the stacked cache, one copy: (2, B, H, 1, D)
-                cache.self_kv[i].index_copy_(3, pos, qkv[..., HD:].view(B, 1, 2, H, D).permute(2, 0, 3, 1, 4))
+                # new key and value -> slot `pos` of the stacked cache, one copy
+                cache.append_stacked(i, qkv[..., HD:].view(B, 1, 2, H, D), pos)
             else:
                 normed = sa.layer_norm(hidden).to(hidden.dtype)
                 q = shape(att.q(normed))
-                cache.self_k[i].index_copy_(2, pos, shape(att.k(normed)))
-                cache.self_v[i].index_copy_(2, pos, shape(att.v(normed)))
-            o = flash_decoding_with_fusing_bias(q, cache.self_k[i], cache.self_v[i], table, causal=True, sm_scale=1.0,
-                                                NUM_BUCKETS=nb, MAX_DISTANCE=md, seqlens_k=seqlens,
-                                                num_splits=self_splits)
+                cache.append(i, shape(att.k(normed)), shape(att.v(normed)), pos)
+            o = cache.attend_self(i, q, table, nb, md, seqlens=seqlens, num_splits=self_splits)
             o = att.o(o.transpose(1, 2).reshape(B, 1, HD))
             if fused:
                 hidden, normed = add_rms_layer_norm(hidden, o, ca.layer_norm.weight, eps, inplace=True)
             else:
                 hidden = hidden + o
                 normed = ca.layer_norm(hidden).to(hidden.dtype)
-            q = shape(catt.q(normed))
-            o = flash_decoding_with_fusing_bias(q, cache.cross_k[i], cache.cross_v[i], None, causal=False,
-                                                sm_scale=1.0, seqlens_k=encoder_seqlens, q_pos_offset=0)
+            o = cache.attend_cross(i, cross(catt.q(normed)), encoder_seqlens)
             o = catt.o(o.transpose(1, 2).reshape(B, 1, HD))
             if fused:
                 hidden, normed = add_rms_layer_norm(hidden, o, ffl.layer_norm.weight, eps, inplace=True)
@@ -544,6 +651,9 @@ class T5Stack(nn.Module):
         t0 = cache.length
         if t0 + M > cache.max_len:
             raise ValueError("decoder cache is full")
+        if cache.beams != 1:
+            raise ValueError("a cache of several beams belongs to decode_step_static")
+        quantized = isinstance(cache, QuantizedDecoderCache)
         hidden = self.embed_tokens(input_ids)
         table = self._table()
         shape = lambda x: x.view(B, M, H, D).transpose(1, 2)
@@ -552,12 +662,10 @@ class T5Stack(nn.Module):
             att = sa.SelfAttention
             normed = sa.layer_norm(hidden).to(hidden.dtype)
             q = shape(att.q(normed))
-            cache.self_k[i][:, :, t0:t0 + M] = shape(att.k(normed))
-            cache.self_v[i][:, :, t0:t0 + M] = shape(att.v(normed))
-            if M <= att.decode_max_rows:
-                o = flash_decoding_with_fusing_bias(q, cache.self_k[i], cache.self_v[i], table, causal=True,
-                                                    sm_scale=1.0, NUM_BUCKETS=cfg.relative_attention_num_buckets,
-                                                    MAX_DISTANCE=cfg.relative_attention_max_distance, kv_len=t0 + M)
+            cache.append(i, shape(att.k(normed)), shape(att.v(normed)), t0)
+            if M <= att.decode_max_rows or quantized:
+                o = cache.attend_self(i, q, table, cfg.relative_attention_num_buckets, cfg.relative_attention_max_distance,
+                                      kv_len=t0 + M)
             else:
                 o = flash_attention_with_fusing_bias(q, cache.self_k[i][:, :, :t0 + M], cache.self_v[i][:, :, :t0 + M],
                                                      table, causal=True, sm_scale=1.0,
@@ -567,9 +675,8 @@ class T5Stack(nn.Module):
             catt = ca.EncDecAttention
             normed = ca.layer_norm(hidden).to(hidden.dtype)
             q = shape(catt.q(normed))
-            if M <= catt.decode_max_rows:
-                o = flash_decoding_with_fusing_bias(q, cache.cross_k[i], cache.cross_v[i], None, causal=False,
-                                                    sm_scale=1.0, seqlens_k=encoder_seqlens, q_pos_offset=0)
+            if M <= catt.decode_max_rows or quantized:
+                o = cache.attend_cross(i, q, encoder_seqlens)
             else:
                 o = flash_attention_with_fusing_bias(q, cache.cross_k[i], cache.cross_v[i], None, causal=False,
                                                      sm_scale=1.0, q_pos_offset=0)
@@ -604,7 +711,8 @@ def _native_decoding(model, encoder_hidden_states, max_len, encoder_seqlens=None
 
 
 class GraphedDecoding:
-    """Greedy generation whose single-token step is one CUDA graph.
+    """Greedy generation whose single-token step is one CUDA graph; `cache_dtype` torch.float8_e4m3fn keeps the
+    keys and values in 8 bits.
 
     The step (all decoder layers, LM head, argmax, token write-back, position update) is run
     once eagerly on a side stream (cuBLAS handles and stacked weights then exist), rewound,
@@ -616,7 +724,7 @@ class GraphedDecoding:
     changes between replays.
     """
 
-    def __init__(self, model, encoder_hidden_states, max_len, encoder_seqlens=None):
+    def __init__(self, model, encoder_hidden_states, max_len, encoder_seqlens=None, cache_dtype=None):
         B = encoder_hidden_states.shape[0]
         dev = encoder_hidden_states.device
         self.model = model
@@ -624,11 +732,15 @@ class GraphedDecoding:
         self.steps_done = 0
         self.encoder_seqlens = encoder_seqlens
         with torch.no_grad():
-            self.session = _native_decoding(model, encoder_hidden_states, max_len, encoder_seqlens)
+            self.session = None
+            if cache_dtype is None:
+                self.session = _native_decoding(model, encoder_hidden_states, max_len, encoder_seqlens)
         if self.session is not None:
             self.tokens, self.last_logits = _host.decode_session_tensors(self.session)
         else:
-            self.cache = model.decoder.new_cache(encoder_hidden_states, max_len)
+            with torch.no_grad():
+                self.cache = model.decoder.new_cache(encoder_hidden_states, max_len, cache_dtype=cache_dtype,
+                                                     encoder_seqlens=encoder_seqlens)
             self.cur = torch.empty((B, 1), dtype=torch.long, device=dev)
             self.pos = torch.empty(1, dtype=torch.long, device=dev)
             self.seqlens = torch.empty(B, dtype=torch.int32, device=dev)
@@ -673,6 +785,96 @@ class GraphedDecoding:
             raise RuntimeError("the cache is full: %d steps" % self.max_len)
         self.graph.replay()
         self.steps_done += 1
+
+
+class BeamDecoding:
+    """Beam search over a preallocated cache; the step is one CUDA graph (`use_cuda_graph=False`: launched one by one).
+
+    A step runs the decoder on a row per beam (the beams of a sentence read its encoder keys together), the LM head,
+    `beam_search_step` and `reorder_beam_cache`; positions, lengths, scores, the pool of finished sentences and the
+    history of tokens and parents live on the device.  `cache_dtype` torch.float8_e4m3fn keeps keys and values in 8 bits.
+    `sequences()` reads the best sentences back from the history at any time.
+    """
+
+    def __init__(self, model, encoder_hidden_states, max_len, num_beams, encoder_seqlens=None, length_penalty=1.0,
+                 early_stopping=False, cache_dtype=None, use_cuda_graph=True):
+        if not 1 <= num_beams <= MAX_BEAMS:
+            raise ValueError("between 1 and %d beams, got %d" % (MAX_BEAMS, num_beams))
+        if max_len < 1:
+            raise ValueError("at least one step, got %d" % max_len)
+        B, dev = encoder_hidden_states.shape[0], encoder_hidden_states.device
+        self.model, self.max_len, self.batch, self.beams = model, max_len, B, num_beams
+        self.encoder_seqlens = encoder_seqlens
+        self.options = dict(eos_token_id=model.cfg.eos_token_id, pad_token_id=model.cfg.pad_token_id,
+                            length_penalty=length_penalty)
+        self.early_stopping = early_stopping
+        with torch.no_grad():
+            self.cache = model.decoder.new_cache(encoder_hidden_states, max_len, num_beams, cache_dtype, encoder_seqlens)
+        if cache_dtype is None:
+            self.cache.own_workspace()
+        shape = (B, num_beams)
+        self.cur = torch.empty(shape, dtype=torch.long, device=dev)
+        self.parents = torch.empty(shape, dtype=torch.int32, device=dev)
+        self.scores = torch.empty(shape, dtype=torch.float32, device=dev)
+        self.finished_scores = torch.empty(shape, dtype=torch.float32, device=dev)
+        self.finished_steps = torch.empty(shape, dtype=torch.int32, device=dev)
+        self.finished_beams = torch.empty(shape, dtype=torch.int32, device=dev)
+        self.done = torch.empty(B, dtype=torch.bool, device=dev)
+        self.history = tuple(torch.empty((max_len, *shape), dtype=torch.int32, device=dev) for _ in range(2))
+        self.pos = torch.empty(1, dtype=torch.long, device=dev)
+        self.seqlens = torch.empty(B * num_beams, dtype=torch.int32, device=dev)
+        self.graph = None
+        self.rewind()
+        if use_cuda_graph:
+            side = torch.cuda.Stream(dev)
+            side.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(side), torch.no_grad():
+                self._step()                             # library handles and stacked weights exist from here on
+            torch.cuda.current_stream(dev).wait_stream(side)
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.graph), torch.no_grad():
+                self._step()
+            self.rewind()
+
+    def rewind(self):
+        """Back to the start of the search."""
+        self.cur.fill_(self.model.cfg.decoder_start_token_id)
+        self.scores.fill_(float("-inf"))
+        self.scores[:, 0] = 0.0                          # the first step goes on from one beam of each sentence
+        self.finished_scores.fill_(float("-inf"))
+        for t in (self.finished_steps, self.finished_beams, self.done, self.pos):
+            t.zero_()
+        self.seqlens.fill_(1)
+        self.steps_done = 0
+
+    def _step(self):
+        m = self.model
+        hidden = m.decoder.decode_step_static(self.cur.view(-1, 1), self.cache, self.pos, self.seqlens, self.encoder_seqlens)
+        state = (self.scores, self.finished_scores, self.finished_steps, self.finished_beams, self.done)
+        beam_search_step(m.logits(hidden), *state, self.pos, early_stopping=self.early_stopping,
+                         out=(self.cur, self.parents, *state), history=self.history, **self.options)
+        self.cache.reorder(self.parents, self.seqlens)
+        self.pos.add_(1)
+        self.seqlens.add_(1)
+
+    def step(self):
+        if self.steps_done >= self.max_len:
+            raise RuntimeError("the cache is full: %d steps" % self.max_len)
+        if self.graph is not None:
+            self.graph.replay()
+        else:
+            with torch.no_grad():
+                self._step()
+        self.steps_done += 1
+
+    def sequences(self, num_return_sequences=1):
+        """(ids (batch, num_return_sequences, steps done), scores) of the best sentences so far."""
+        if self.steps_done == 0:
+            raise RuntimeError("no step has been made")
+        tokens, parents = (h[:self.steps_done] for h in self.history)
+        return beam_search_sequences(tokens, parents, self.scores, self.finished_scores, self.finished_steps,
+                                     self.finished_beams, self.done, num_return_sequences=num_return_sequences,
+                                     **self.options)
 
 
 class GraphedForward:
@@ -777,10 +979,16 @@ class T5ForConditionalGeneration(nn.Module):
         return graphs[key](input_ids, decoder_input_ids)
 
     @torch.no_grad()
-    def generate(self, input_ids, attention_mask=None, max_new_tokens=32, use_cuda_graph=True):
-        """Greedy generation for a (padded) batch of prompts: the encoder pass on the packed valid tokens
+    def generate(self, input_ids, attention_mask=None, max_new_tokens=32, use_cuda_graph=True, num_beams=1,
+                 length_penalty=1.0, early_stopping=False, num_return_sequences=1, cache_dtype=None):
+        """Generation for a (padded) batch of prompts: the encoder pass on the packed valid tokens
         (`forward_fused`), the cross-attention keys and values projected once into the preallocated cache,
-        then one captured single-token step per new token.  Returns the generated ids (B, max_new_tokens)."""
+        then one captured single-token step per new token.  Greedy, or with `num_beams` > 1 the best sentence of a beam
+        search (`beam_search`, which takes the options after it).  `cache_dtype` torch.float8_e4m3fn keeps keys and values
+        in 8 bits.  Returns the generated ids (B, max_new_tokens); (B, num_return_sequences, max_new_tokens) with more than
+        one sentence."""
+        if num_beams == 1 and num_return_sequences != 1:
+            raise ValueError("greedy generation has one sentence to return")
         fused = self.cfg.attention_type == "flash" and input_ids.is_cuda and \
             self.shared.weight.dtype in (torch.bfloat16, torch.float16)
         seqlens = None
@@ -790,29 +998,55 @@ class T5ForConditionalGeneration(nn.Module):
             enc = self.encoder.forward_fused(input_ids, attention_mask=attention_mask)
         else:
             enc = self.encoder(input_ids, attention_mask=attention_mask)
-        tokens, _ = self.greedy_decode(enc, max_new_tokens, encoder_seqlens=seqlens, use_cuda_graph=use_cuda_graph)
+        if num_beams > 1:
+            tokens, _ = self.beam_search(enc, max_new_tokens, num_beams, encoder_seqlens=seqlens, length_penalty=length_penalty,
+                                         early_stopping=early_stopping, num_return_sequences=num_return_sequences,
+                                         cache_dtype=cache_dtype, use_cuda_graph=use_cuda_graph)
+            return tokens[:, 0] if num_return_sequences == 1 else tokens
+        tokens, _ = self.greedy_decode(enc, max_new_tokens, encoder_seqlens=seqlens, use_cuda_graph=use_cuda_graph,
+                                       cache_dtype=cache_dtype)
         return tokens
 
     @torch.no_grad()
-    def greedy_decode(self, encoder_hidden_states, steps, encoder_seqlens=None, use_cuda_graph=False):
+    def beam_search(self, encoder_hidden_states, steps, num_beams, encoder_seqlens=None, length_penalty=1.0,
+                    early_stopping=False, num_return_sequences=1, cache_dtype=None, use_cuda_graph=True):
+        """Beam search from `decoder_start_token_id` (`BeamDecoding`): (ids (B, num_return_sequences, steps), scores
+        (B, num_return_sequences)), best first, `pad_token_id` behind the end of a sentence.  A sentence's score is its
+        log-probability over its length to the power of `length_penalty`; `early_stopping` ends a search as soon as
+        num_beams sentences are finished.  Whether all searches have ended is looked up every 16 steps."""
+        search = BeamDecoding(self, encoder_hidden_states, steps, num_beams, encoder_seqlens, length_penalty, early_stopping,
+                              cache_dtype, use_cuda_graph)
+        for t in range(steps):
+            search.step()
+            if t % 16 == 15 and bool(search.done.all()):
+                break
+        tokens, scores = search.sequences(num_return_sequences)
+        return nn.functional.pad(tokens, (0, steps - tokens.shape[-1]), value=self.cfg.pad_token_id), scores
+
+    @torch.no_grad()
+    def greedy_decode(self, encoder_hidden_states, steps, encoder_seqlens=None, use_cuda_graph=False, cache_dtype=None):
         """Greedy generation from `decoder_start_token_id` with the preallocated cache.
 
-        Where the native step kernels cover the model (16-bit plain stacks, up to 64 rows) every token is one
-        native launch chain.  Otherwise, with `use_cuda_graph`, the whole single-token step (all layers, LM
-        head, argmax, position update) is captured once after a warm-up step and replayed: one graph
-        launch per token instead of a few hundred kernel launches issued from Python.
+        Where the native step kernels cover the model (16-bit plain stacks, up to 64 rows, a cache in the model's
+        type) every token is one native launch chain.  Otherwise, with `use_cuda_graph`, the whole single-token step
+        (all layers, LM head, argmax, position update) is captured once after a warm-up step and replayed: one graph
+        launch per token instead of a few hundred kernel launches issued from Python.  `cache_dtype`
+        torch.float8_e4m3fn keeps keys and values in 8 bits.
         """
-        session = _native_decoding(self, encoder_hidden_states, steps, encoder_seqlens)
+        session = None
+        if cache_dtype is None:
+            session = _native_decoding(self, encoder_hidden_states, steps, encoder_seqlens)
         if session is not None:
             _host.decode_session_run(session, steps)
             return _host.decode_session_tensors(session)
         if use_cuda_graph:
-            session = GraphedDecoding(self, encoder_hidden_states, steps, encoder_seqlens)
+            session = GraphedDecoding(self, encoder_hidden_states, steps, encoder_seqlens, cache_dtype)
             for _ in range(steps):
                 session.step()
             return session.tokens, session.last_logits
         B = encoder_hidden_states.shape[0]
-        cache = self.decoder.new_cache(encoder_hidden_states, steps)
+        cache = self.decoder.new_cache(encoder_hidden_states, steps, cache_dtype=cache_dtype,
+                                       encoder_seqlens=encoder_seqlens)
         cur = torch.full((B, 1), self.cfg.decoder_start_token_id, dtype=torch.long, device=encoder_hidden_states.device)
         tokens, last_logits = [], None
         for _ in range(steps):
