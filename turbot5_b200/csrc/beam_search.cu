@@ -86,6 +86,20 @@ __device__ __forceinline__ double score_of(const Row& r, float x) {
   return s == s ? s : -(double)INFINITY;
 }
 
+// ln x for 1 <= x < 2^60 to about 1e-13: x = 2^e f, f in [0.7, 1.42), ln f = 2 artanh((f - 1) / (f + 1)) by its series.
+__device__ __forceinline__ double log_of(double x) {
+  int64_t bits = __double_as_longlong(x);
+  int e = (int)(bits >> 52) - 1023;
+  double f = __longlong_as_double((bits & 0xfffffffffffffll) | 0x3ff0000000000000ll);
+  if (f > 1.4142135623730951) { f *= 0.5; ++e; }
+  double r = (double)__frcp_rn((float)(f + 1.0));        // 1 / (f + 1): 24 bits, doubled once
+  r = r * (2.0 - (f + 1.0) * r);
+  const double s = (f - 1.0) * r, q = s * s, q2 = q * q, q4 = q2 * q2;
+  const double even = (1.0 + q * (1.0 / 3)) + q2 * (1.0 / 5 + q * (1.0 / 7));
+  const double odd = (1.0 / 9 + q * (1.0 / 11)) + q2 * (1.0 / 13 + q * (1.0 / 15));
+  return e * 0.6931471805599453 + 2.0 * s * (even + q4 * odd);
+}
+
 template <typename T> struct Pack;
 template <> struct Pack<float> { static constexpr int N = 4; static constexpr uint32_t none = 0xff800000u; };
 template <> struct Pack<__half> { static constexpr int N = 8; static constexpr uint32_t none = 0xfc00fc00u; };
@@ -213,24 +227,27 @@ __device__ __noinline__ uint64_t best_of_slice(const Slice<T>& sl, int beam, int
 struct Shared {
   double usum[MAX_UNITS];
   float umax[MAX_UNITS];
+  float reached[MAX_UNITS];              // what n elements of a segment reach, at its first slice (-inf elsewhere)
   alignas(16) float group[THREADS];      // maxima of groups of lanes, a segment's from its first warp's place on
   float bound[WARPS];                    // found by this warp; the smallest of a segment's holds
   Row rows[MAX_BEAMS];                   // running rows, in order
   double inv_length;
   int counts[MAX_CLUSTER];               // candidates found by each block
   int found_here, overflow, kept;
+  uint32_t threshold;                    // a score that n candidates reach, ordered bits of a float
   union {
     struct {
       uint64_t found[MAX_FOUND];         // their keys
-      double score[MAX_FOUND + 64];      // scores and keys, one candidate behind the other, padded
-      uint64_t key[MAX_FOUND + 64];
+      double score[MAX_FOUND];           // scores and keys, one candidate behind the other
+      uint64_t key[MAX_FOUND];
     };
     struct {
       uint64_t lists[WARPS][32];
       Cand heads[WARPS];
     };
   };
-  Cand best[FEW];
+  Cand best[FEW];                        // candidates that are left
+  Cand chosen[2][2 * MAX_BEAMS];         // the n best in order, for each of the warps that decide
 };
 
 // The n-th largest of a segment's group maxima: a value that at least n of its elements reach (-inf where too few groups
@@ -240,10 +257,12 @@ __device__ __noinline__ float segment_bound(Shared& sm, float mine, int n, int w
   if (shift > 0) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
   if (shift > 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
   if (shift > 2) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 4));
+  if (shift > 3) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 8));
   const int groups = warps * 32 >> shift, at = first * 32, here = warp - first;
   if ((lane & ((1 << shift) - 1)) == 0) sm.group[at + ((here * 32 + lane) >> shift)] = mine;
   __syncthreads();
-  // four threads per group, as far as the segment has them (a group each otherwise)
+  // four threads per group, as far as the segment has them (a group each otherwise); up to three groups that do not fill a
+  // vector are not counted, which can only lower the bound
   const int share = warps > 7 ? 2 : 0, t = here * 32 + lane, g = t >> share;
   if (here << 5 < groups << share) {
     const float own = g < groups ? sm.group[at + g] : -INFINITY;
@@ -266,8 +285,12 @@ __device__ __noinline__ float segment_bound(Shared& sm, float mine, int n, int w
   for (int i = 1; i << 5 < groups << share; ++i) least = fminf(least, sm.bound[first + i]);
   return least;
 }
-// lanes per group (their logarithm) so that 33 to 64 groups come out, 32 of a single warp
-__device__ __forceinline__ int group_shift(int warps) { return warps > 8 ? 3 : warps > 4 ? 2 : warps > 2 ? 1 : 0; }
+// lanes per group (their logarithm) so that 33 to 64 groups come out, 17 to 32 for few candidates (8 of 32 groups leave
+// 9.2 elements on average, 8 of 64 leave 8.5), 32 of a single warp
+__device__ __forceinline__ int group_shift(int warps, int n) {
+  const int shift = warps > 8 ? 3 : warps > 4 ? 2 : warps > 2 ? 1 : 0;
+  return n <= 8 && warps > 1 ? shift + 1 : shift;
+}
 
 // What the step decides from its n best candidates, best first; a warp each, lane i has candidate i.
 struct Pool { float score; int step, beam; };
@@ -402,7 +425,7 @@ step_kernel(const __grid_constant__ Params p) {
   Shared* lead = cluster.map_shared_rank(&sm, 0);
   const bool active = owns && run > -INFINITY;
   float m = -INFINITY;
-  if (tid == 0) { sm.found_here = 0; sm.overflow = 0; sm.kept = 0; }
+  if (tid == 0) { sm.found_here = 0; sm.overflow = 0; sm.kept = 0; sm.threshold = 0; }
   if (tid < MAX_CLUSTER) sm.counts[tid] = 0;
   if (active) {
     m = fmaxf(fmaxf(x_head, x_tail), -INFINITY);         // (NaN only: -inf)
@@ -452,9 +475,11 @@ step_kernel(const __grid_constant__ Params p) {
   // ---- the candidates of this block's segments
   const int first = active ? max(k * S - rank * WARPS, 0) : warp;                    // the segment's warps
   const int warps = active ? min((k + 1) * S - rank * WARPS, WARPS) - first : 1;
-  const float least = fmaxf(segment_bound(sm, m, n, warp, lane, first, warps, group_shift(warps)), Lowest<T>::value);
+  const float reached = segment_bound(sm, m, n, warp, lane, first, warps, group_shift(warps, n));
+  const float least = fmaxf(reached, Lowest<T>::value);
   const int share = MAX_FOUND >> p.cluster_log2;
   if (active) {
+    if (lane == 0) lead->reached[unit] = warp == first ? reached : -INFINITY;
     const bool mine = m >= least;
     const uint32_t flagged = __ballot_sync(0xffffffffu, mine);
     // the elements among a lane's vectors that reach the bound: bits, then one after the other (small code on purpose:
@@ -527,8 +552,16 @@ step_kernel(const __grid_constant__ Params p) {
         if (um == most) sum += sm.usum[warp * S + i];
         else if (most < INFINITY && um > -INFINITY) sum += sm.usum[warp * S + i] * (double)fast_exp2((um - most) * kLog2e);
       }
-      sum = log(warp_sum(sum));
-      if (lane == 0) sm.rows[warp] = Row{row_run, (double)most + sum, sum, !(most > -INFINITY) ? 1 : most == INFINITY ? 2 : 0};
+      float reach = -INFINITY;
+      #pragma unroll 1
+      for (int i = most > -INFINITY ? lane : S; i < S; i += 32) reach = fmaxf(reach, sm.reached[warp * S + i]);
+      reach = warp_max(reach);
+      sum = log_of(warp_sum(sum));
+      if (lane == 0) {
+        const Row r{row_run, (double)most + sum, sum, !(most > -INFINITY) ? 1 : most == INFINITY ? 2 : 0};
+        sm.rows[warp] = r;
+        atomicMax(&sm.threshold, ordered(__double2float_rd(score_of(r, reach))));
+      }
     }
     if (warp == WARPS - 1 && lane == 1) {                // (K = 16: this warp has a row as well)
       const double steps = (double)(pos + 1);
@@ -544,7 +577,7 @@ step_kernel(const __grid_constant__ Params p) {
       total += c;
     }
     __syncthreads();
-    int valid = 0;
+    const double threshold = (double)unordered(sm.threshold);
     if (fits) {
       // warps take the blocks' lists in turn
       const int r = warp & (C - 1), step = WARPS * 32 >> p.cluster_log2;
@@ -553,55 +586,55 @@ step_kernel(const __grid_constant__ Params p) {
         const uint64_t key = sm.found[r * share + i];
         const double score = score_of(sm.rows[key_beam(key)], key_logit(key));
         sm.score[before + i] = score; sm.key[before + i] = key;
-        valid += score > -INFINITY;
+        if (score >= threshold && score > -INFINITY) {
+          const int at = atomicAdd(&sm.kept, 1);
+          if (at < FEW) sm.best[at] = Cand{score, key};
+        }
       }
     }
-    if (tid < 64 && fits) { sm.score[total + tid] = -INFINITY; sm.key[total + tid] = 0; }
-    valid = __reduce_add_sync(0xffffffffu, valid);
-    if (lane == 0 && valid) atomicAdd(&sm.kept, valid);
     __syncthreads();
-    bool done = fits && sm.kept >= n;
-    __syncthreads();
-    int count = total;
-    if (done && total > FEW) {
-      // many: the same bound again, over the candidates (thread t has candidates t / 8 + 64 * (t % 8) and 512 further on)
+    int count = sm.kept;
+    bool done = fits && count >= n;
+    if (done && count > FEW) {
+      // many: the bound of a segment again, over all candidates (thread t has candidates t / 8 + 64 * (t % 8) and 512
+      // further on)
       const int i0 = (tid >> 3) + 64 * (tid & 7), i1 = i0 + THREADS;
       const float f0 = i0 < total ? __double2float_rd(sm.score[i0]) : -INFINITY;
       const float f1 = i1 < total ? __double2float_rd(sm.score[i1]) : -INFINITY;
-      if (tid == 0) sm.kept = 0;
       const float least = segment_bound(sm, fmaxf(f0, f1), n, warp, lane, 0, WARPS, 3);
+      if (tid == 0) sm.kept = 0;
+      __syncthreads();
       if (f0 >= least && f0 > -INFINITY) { const int i = atomicAdd(&sm.kept, 1); if (i < FEW) sm.best[i] = Cand{sm.score[i0], sm.key[i0]}; }
       if (f1 >= least && f1 > -INFINITY) { const int i = atomicAdd(&sm.kept, 1); if (i < FEW) sm.best[i] = Cand{sm.score[i1], sm.key[i1]}; }
       __syncthreads();
       count = sm.kept;
       done = count >= n && count <= FEW;
-      if (done && tid < FEW + 64) {
-        const Cand c = tid < count ? sm.best[tid] : Cand{-INFINITY, 0};
-        sm.score[tid] = c.score; sm.key[tid] = c.key;
-      }
-      __syncthreads();
     }
     if (done) {
       asm volatile("barrier.cluster.arrive.relaxed.aligned;");               // the others may go: nothing more reaches them
-      // 4 to 16 threads count for each of the candidates, four comparisons at a time
-      const int team_log2 = count <= 32 ? 4 : count <= 64 ? 3 : 2, team = 1 << team_log2, i = tid >> team_log2;
-      if (i < count) {
-        const double score = sm.score[i];
-        const uint64_t key = sm.key[i];
+      if (count <= 32) {
+        // two warps, each for itself: lane i counts for candidate i, then one sees to the beams and one to the pool
+        if (warp > 1) return;
+        const Cand mine = lane < count ? sm.best[lane] : Cand{-INFINITY, 0};
         int above = 0;
-        #pragma unroll 1
-        for (int j = tid & (team - 1); j < count; j += 4 * team) {
-          #pragma unroll
-          for (int o = 0; o < 4; ++o) above += better(sm.score[j + o * team], sm.key[j + o * team], score, key);
-        }
-        // (teams that share a warp are all in or all out only up to the last one: only its lanes take part)
-        const unsigned lanes = ((1u << team) - 1) << (lane & -team);
-        for (int o = 1; o < team; o <<= 1) above += __shfl_xor_sync(lanes, above, o);
-        if ((tid & (team - 1)) == 0 && above < n) sm.best[above] = Cand{score, key};
+        #pragma unroll 4
+        for (int j = 0; j < count; ++j) above += better(sm.best[j].score, sm.best[j].key, mine.score, mine.key);
+        if (lane < count && above < n) sm.chosen[warp][above] = mine;
+        __syncwarp();
+      } else {
+        // four threads count for each of the candidates
+        const int i = tid >> 2;
+        const Cand mine = i < count ? sm.best[i] : Cand{-INFINITY, 0};
+        int above = 0;
+        #pragma unroll 2
+        for (int j = tid & 3; j < count; j += 4) above += better(sm.best[j].score, sm.best[j].key, mine.score, mine.key);
+        above += __shfl_xor_sync(0xffffffffu, above, 1);
+        above += __shfl_xor_sync(0xffffffffu, above, 2);
+        if (i < count && (tid & 3) < 2 && above < n) sm.chosen[tid & 1][above] = mine;
+        __syncthreads();
       }
-      __syncthreads();
-      if (warp == 0) go_on(p, sm.best, b, lane, pos);
-      if (warp == 1) settle(p, sm.best, b, lane, pool, pos, sm.inv_length);
+      if (warp == 0) go_on(p, sm.chosen[0], b, lane, pos);
+      if (warp == 1) settle(p, sm.chosen[1], b, lane, pool, pos, sm.inv_length);
       return;
     }
     if (tid < C) cluster.map_shared_rank(&sm, tid)->overflow = 1;
@@ -634,12 +667,12 @@ step_kernel(const __grid_constant__ Params p) {
       top = sm.heads[0];
       #pragma unroll 1
       for (int w = 1; w < WARPS; ++w) if (better(sm.heads[w].score, sm.heads[w].key, top.score, top.key)) top = sm.heads[w];
-      if (tid == 0) sm.best[i] = top;
+      if (tid < 2) sm.chosen[tid][i] = top;
       if (mine.key && mine.key == top.key) { ++next; take(); }
       __syncthreads();
     }
-    if (warp == 0) go_on(p, sm.best, b, lane, pos);
-    if (warp == 1) settle(p, sm.best, b, lane, pool, pos, sm.inv_length);
+    if (warp == 0) go_on(p, sm.chosen[0], b, lane, pos);
+    if (warp == 1) settle(p, sm.chosen[1], b, lane, pool, pos, sm.inv_length);
   }
   cluster.sync();                        // nobody leaves while its shared memory is read
 }
