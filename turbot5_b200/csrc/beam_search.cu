@@ -424,7 +424,9 @@ step_kernel(const __grid_constant__ Params p) {
   // ---- one pass over the logits: maximum and sum of exponentials of a slice
   Shared* lead = cluster.map_shared_rank(&sm, 0);
   const bool active = owns && run > -INFINITY;
-  float m = -INFINITY;
+  // a lane's maximum, its vector with the largest element and what its other vectors reach at most
+  float m = -INFINITY, in_best = -INFINITY, in_others = -INFINITY;
+  int best_at = 0;
   if (tid == 0) { sm.found_here = 0; sm.overflow = 0; sm.kept = 0; sm.threshold = 0; }
   if (tid < MAX_CLUSTER) sm.counts[tid] = 0;
   if (active) {
@@ -439,8 +441,12 @@ step_kernel(const __grid_constant__ Params p) {
         if (v + 32 * i < sl.v1) {        // (the same for the whole warp)
           float x[N];
           unpack<T>(u[i], x);
+          float most = -INFINITY;
           #pragma unroll
-          for (int e = 0; e < N; e += 4) m_new = fmaxf(m_new, fmaxf(fmaxf(x[e], x[e + 1]), fmaxf(x[e + 2], x[e + 3])));
+          for (int e = 0; e < N; e += 4) most = fmaxf(most, fmaxf(fmaxf(x[e], x[e + 1]), fmaxf(x[e + 2], x[e + 3])));
+          in_others = fmaxf(in_others, fminf(in_best, most));
+          if (most > in_best) { in_best = most; best_at = v + 32 * i; }
+          m_new = fmaxf(m_new, most);
         }
       const float ref = m_new > -INFINITY ? m_new : 0.f;
       s *= fast_exp2((m - ref) * kLog2e);
@@ -481,7 +487,6 @@ step_kernel(const __grid_constant__ Params p) {
   if (active) {
     if (lane == 0) lead->reached[unit] = warp == first ? reached : -INFINITY;
     const bool mine = m >= least;
-    const uint32_t flagged = __ballot_sync(0xffffffffu, mine);
     // the elements among a lane's vectors that reach the bound: bits, then one after the other (small code on purpose:
     // what runs once per launch pays its way through the instruction cache)
     auto push = [&](float x, int token) {
@@ -492,46 +497,36 @@ step_kernel(const __grid_constant__ Params p) {
       if (x_head >= least) push(x_head, lane);
       if (x_tail >= least) push(x_tail, sl.tail + lane);
     }
-    const bool in_registers = sl.v1 - sl.v0 <= 32 * U;   // the whole slice is still there
-    uint32_t todo = in_registers ? (flagged ? 1u : 0u) : flagged;
-    #pragma unroll 1
-    for (; todo; ) {
-      // from registers, all flagged lanes at once; else the vectors of up to four flagged lanes again, eight lanes for
-      // each, four vectors a lane
-      int base = sl.v0 + lane, stride = 32;
-      bool look = mine;
-      if (!in_registers) {
-        uint32_t t = todo;
-        #pragma unroll 1
-        for (int i = lane >> 3; i > 0; --i) t &= t - 1;
-        look = t != 0;
-        base = sl.v0 + __ffs(t) - 1 + 32 * (lane & 7); stride = 32 * 8;
-        todo &= todo - 1; todo &= todo - 1; todo &= todo - 1; todo &= todo - 1;
-      } else {
-        todo = 0;
-      }
+    auto push_vector = [&](const uint4& w, int v) {
+      const uint4 one[1] = {w};
       #pragma unroll 1
-      for (; __any_sync(0xffffffffu, look && base < sl.v1); base += stride * U) {
-        if (!in_registers) {
-          #pragma unroll
-          for (int i = 0; i < U; ++i)
-            u[i] = look && base + stride * i < sl.v1 ? __ldg(sl.mid + base + stride * i)
-                                                     : make_uint4(Pack<T>::none, Pack<T>::none, Pack<T>::none, Pack<T>::none);
-        }
-        uint32_t mask = look ? mask_of<T, U>(u, least) : 0;
-        #pragma unroll 1
-        for (; mask; mask &= mask - 1) {
-          const int bit = __ffs(mask) - 1, q = bit & 15, i = q >> 2, e = N == 8 ? 2 * (q & 3) + (bit >> 4) : q & 3;
-          uint4 w = u[0];
-          #pragma unroll
-          for (int j = 1; j < U; ++j) if (i == j) w = u[j];
-          float x[N], found = 0.f;
-          unpack<T>(w, x);
-          #pragma unroll
-          for (int j = 0; j < N; ++j) if (e == j) found = x[j];
-          push(found, sl.first + (base + stride * i) * N + e);
-        }
+      for (uint32_t mask = mask_of<T, 1>(one, least); mask; mask &= mask - 1) {
+        const int bit = __ffs(mask) - 1, e = N == 8 ? 2 * (bit & 3) + (bit >> 4) : bit & 3;
+        float x[N], found = 0.f;
+        unpack<T>(w, x);
+        #pragma unroll
+        for (int j = 0; j < N; ++j) if (e == j) found = x[j];
+        push(found, sl.first + v * N + e);
       }
+    };
+    // most lanes have one vector that reaches the bound: still in registers where the slice is four vectors a lane
+    const bool one = mine && in_best >= least && in_others < least;
+    if (__any_sync(0xffffffffu, one)) {
+      uint4 w = u[0];
+      if (sl.v1 - sl.v0 <= 32 * U) {
+        #pragma unroll
+        for (int j = 1; j < U; ++j) if (best_at == sl.v0 + 32 * j) w = u[j];
+      } else if (one) {
+        w = __ldg(sl.mid + best_at + lane);
+      }
+      if (one) push_vector(w, best_at + lane);
+    }
+    #pragma unroll 1
+    for (uint32_t todo = __ballot_sync(0xffffffffu, mine && in_others >= least); todo; todo &= todo - 1) {
+      const int who = __ffs(todo) - 1;                   // several: its vectors again, by the whole warp
+      #pragma unroll 1
+      for (int v = sl.v0 + who + 32 * lane; v < sl.v1; v += 32 * 32) push_vector(__ldg(sl.mid + v), v);
+      __syncwarp();
     }
   }
   __syncthreads();
