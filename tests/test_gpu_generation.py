@@ -321,6 +321,18 @@ def test_reorder_views_many_tensors_and_scales():
         assert torch.equal(s[..., :2], s0[:, rows][..., :2]) and torch.equal(s[..., 2:], s0[..., 2:])
 
 
+def test_reorder_single_tokens_and_numbers():
+    """Dimensions of size one may have any stride."""
+    import turbot5_b200 as t5b
+    parents = torch.tensor([[1, 0, 0]], dtype=torch.int32, device="cuda")
+    for shape, order in (((3, 2, 1, 8), (0, 1, 3, 2)), ((3, 2, 5, 1), (0, 1, 2, 3))):
+        base = torch.arange(48, device="cuda", dtype=torch.float32)[:math.prod(shape)]
+        cache = base.view(*(shape[i] for i in order)).permute(*(order.index(i) for i in range(4)))
+        want = cache[[1, 0, 0]].clone()
+        t5b.reorder_beam_cache([cache], parents)
+        assert torch.equal(cache, want)
+
+
 def test_reorder_lengths_outside_the_cache():
     import turbot5_b200 as t5b
     cache = torch.arange(2 * 4 * 8, device="cuda", dtype=torch.float32).view(2, 1, 4, 8).contiguous()
@@ -620,6 +632,9 @@ def test_refusals_on_the_device():
         step(logits, *dev, pos, length_penalty=float("nan"))
     with pytest.raises(ValueError):
         step(logits, *dev, pos, out=dev)
+    twice = [torch.empty((2, 4), dtype=torch.long, device="cuda"), dev[2], *dev]
+    with pytest.raises(ValueError, match="same"):
+        step(logits, *dev, pos, out=twice)
     with pytest.raises((TypeError, ValueError)):
         step(logits, *dev, pos, history=[torch.zeros((3, 2, 4), device="cuda")] * 2)
     hist = torch.zeros((3, 2, 4), dtype=torch.int32, device="cuda")
@@ -655,6 +670,8 @@ def test_refusals_on_the_device():
                        ((q, k, ks, v, vs, table[:20]), ValueError), ((q, k.float(), ks, v, vs, None), TypeError)):
         with pytest.raises(error):
             att(*bad)
+    with pytest.raises(RuntimeError):
+        att(q, k, ks, v, vs, None, q_pos_offset=0x7fffffff - 100)
     for kw in (dict(kv_len=129), dict(kv_len=-1), dict(seqlens_k=torch.zeros(3, dtype=torch.int32, device="cuda"))):
         with pytest.raises(ValueError):
             att(q, k, ks, v, vs, None, **kw)

@@ -820,26 +820,27 @@ sequences_kernel(const __grid_constant__ SequenceParams p) {
   }
 }
 
-static int cluster_blocks(int B, int K, int64_t bytes) {
+static int cluster_blocks(int B, int K, int64_t bytes, int most) {
   // Two blocks per multiprocessor keep the whole batch resident; more blocks per sentence shorten its pass, 16 only where
   // a slice would not fit a warp's registers with 8 (a sentence of 4 x 32128 16-bit logits: 7.9 us with 8, 8.5 with 16;
   // of 16 x 65537 float32: 26.7 and 21.6).  A beam has two warps at least, for the number of groups that its bound is
   // taken from.
-  int C = bytes > 8 * WARPS * 32 * 4 * 16 ? 16 : 8;
+  int C = bytes > 8 * WARPS * 32 * 4 * 16 ? most : 8;
   while (C > (K > 8 ? 2 : 1) && (long long)B * C > (C == 16 ? 148 : 2 * 148)) C /= 2;
   return C;
 }
 
 template <typename T>
 static int launch_step(Params p, cudaStream_t stream) {
-  static std::atomic<bool> wide[64];     // per device: clusters of 16 are allowed for this kernel (setting it twice is harmless)
+  static std::atomic<int> most[64];      // per device: the largest cluster this kernel can have (found twice, it is the same)
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return T5B_ERR_LAUNCH;
-  if (!wide[dev]) {
-    if (cudaFuncSetAttribute(step_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return T5B_ERR_LAUNCH;
-    wide[dev] = true;
+  if (!most[dev]) {
+    const int found = largest_cluster((const void*)step_kernel<T>, THREADS, 0);
+    if (found == 0) return T5B_ERR_LAUNCH;
+    most[dev] = found;
   }
-  const int C = cluster_blocks(p.B, p.K, (int64_t)p.K * p.V * sizeof(T));
+  const int C = cluster_blocks(p.B, p.K, (int64_t)p.K * p.V * sizeof(T), most[dev]);
   for (p.cluster_log2 = 0; 1 << p.cluster_log2 < C;) ++p.cluster_log2;
   p.S = C * WARPS / p.K;
   p.unit_magic = (65536u + p.S - 1) / p.S; p.slice_magic = (uint32_t)(((1ull << 32) + p.S - 1) / p.S);

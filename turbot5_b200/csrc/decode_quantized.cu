@@ -460,15 +460,17 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
 template <typename T, int D, int TILES, int WARPS>
 static int launch(const Params& p, const BucketSpec& spec, int C, cudaStream_t stream) {
   constexpr int smem = WARPS * Ring<D>::WARP_BYTES;
-  static std::atomic<bool> ready[64];    // per device: more shared memory, clusters of 16 (setting them twice is harmless)
+  static std::atomic<int> most[64];      // per device: the largest cluster this kernel can have (found twice, it is the same)
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return T5B_ERR_LAUNCH;
-  if (!ready[dev]) {
+  if (!most[dev]) {
     const auto kernel = decode_quantized_kernel<T, D, TILES, WARPS>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return T5B_ERR_LAUNCH;
-    ready[dev] = true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return T5B_ERR_LAUNCH;
+    const int found = largest_cluster((const void*)kernel, WARPS * 32, smem);
+    if (found == 0) return T5B_ERR_LAUNCH;
+    most[dev] = found;
   }
+  if (C > most[dev]) C = most[dev];
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)C, (unsigned)p.H, (unsigned)(p.B * p.row_groups));
   cfg.blockDim = dim3(WARPS * 32); cfg.stream = stream; cfg.dynamicSmemBytes = smem;
@@ -525,8 +527,9 @@ extern "C" int t5b_decode_quantized_fwd(const t5b_decode_quantized_args* a, void
   if (!a) return T5B_ERR_ARG;
   if (a->dtype != T5B_F16 && a->dtype != T5B_BF16) return T5B_ERR_DTYPE;
   if (a->D != 16 && a->D != 32 && a->D != 64 && a->D != 128) return T5B_ERR_HEAD_DIM;
-  if (a->B < 0 || a->H < 0 || a->M < 0 || a->N < 0 || a->H > 65535) return T5B_ERR_SHAPE;
+  if (a->B < 0 || a->H < 0 || a->M < 0 || a->N < 0 || a->H > 65535 || a->M > (1 << 20)) return T5B_ERR_SHAPE;
   if (a->B == 0 || a->H == 0 || a->M == 0) return T5B_OK;
+  if (a->q_pos_offset > 0x7fffffff - a->M - 2 * T5B_CACHE_BLOCK) return T5B_ERR_ARG;      // positions are 32-bit numbers
   if (!a->q || !a->out || (a->N > 0 && (!a->k || !a->v || !a->k_scale || !a->v_scale))) return T5B_ERR_ARG;
   if ((uintptr_t)a->k % 16 || (uintptr_t)a->v % 16 || (uintptr_t)a->q % 2 || (uintptr_t)a->k_scale % 4 || (uintptr_t)a->v_scale % 4)
     return T5B_ERR_ALIGN;

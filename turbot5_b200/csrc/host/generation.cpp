@@ -106,6 +106,9 @@ PyObject* py_beam_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       else check_plain(out[i], types[i], bk, dev, names[i]);
     }
   }
+  for (int i = 0; i < 7; ++i)
+    for (int j = 0; j < i; ++j)
+      TORCH_CHECK_VALUE(B == 0 || out[i].data_ptr() != out[j].data_ptr(), "two of the tensors in out are the same");
   std::vector<Tensor> history;
   int64_t steps = 0;
   if (a[12] != Py_None) {
@@ -189,7 +192,8 @@ Rows rows_of(const std::vector<Tensor>& ts, int64_t dims, int64_t R, at::Device 
   TORCH_CHECK_VALUE(t0.defined() && (t0.dim() == dims || t0.dim() == dims + 1), name, " must have ", dims, " or ", dims + 1, " dimensions");
   const int64_t d = t0.dim() - dims, es = t0.element_size();
   TORCH_CHECK_VALUE(t0.size(d) == R, name, " must have batch * num_beams = ", R, " rows, got ", t0.size(d));
-  TORCH_CHECK_VALUE(t0.numel() == 0 || (t0.stride(-1) == 1 && (dims == 3 || t0.stride(-2) == t0.size(-1))),
+  TORCH_CHECK_VALUE(t0.numel() == 0 || ((t0.size(-1) == 1 || t0.stride(-1) == 1) &&
+                                        (dims == 3 || t0.size(-2) == 1 || t0.stride(-2) == t0.size(-1))),
                     name, ": a head's tokens must lie one behind the other");
   if (d == 1) { r.outer = t0.size(0); r.outer_stride = t0.stride(0) * es; }
   r.row_stride = t0.stride(d) * es; r.head_stride = t0.stride(d + 1) * es;
