@@ -268,21 +268,29 @@ __device__ __noinline__ float segment_bound(Shared& sm, float mine, int n, int w
     const float own = g < groups ? sm.group[at + g] : -INFINITY;
     int above = 0;
     const float4* every = (const float4*)(sm.group + at);
-    #pragma unroll 4
-    for (int j = t & ((1 << share) - 1); j < groups / 4; j += 1 << share) {
-      const float4 o = every[j];
-      above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
-    }
-    if (share) {
+    auto count = [&](const float4& o) { above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own); };
+    if (share) {                         // at most 16 vectors, four a thread, read together
+      float4 o[4];
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = (t & 3) + 4 * i;
+        o[i] = j < groups / 4 ? every[j] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      }
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) count(o[i]);
       above += __shfl_xor_sync(0xffffffffu, above, 1);
       above += __shfl_xor_sync(0xffffffffu, above, 2);
+    } else {
+      #pragma unroll 4
+      for (int j = 0; j < groups / 4; ++j) count(every[j]);
     }
     const float least = -warp_max(above < n && g < groups ? -own : -INFINITY);
     if (lane == 0) sm.bound[warp] = least;
   }
   __syncthreads();
   float least = sm.bound[first];
-  for (int i = 1; i << 5 < groups << share; ++i) least = fminf(least, sm.bound[first + i]);
+  #pragma unroll
+  for (int i = 1; i < 8; ++i) least = fminf(least, i << 5 < groups << share ? sm.bound[first + i] : INFINITY);
   return least;
 }
 // lanes per group (their logarithm) so that 33 to 64 groups come out, 17 to 32 for few candidates (8 of 32 groups leave
