@@ -361,6 +361,7 @@ __device__ __forceinline__ void go_on(const Params& p, const Cand* best, int b, 
   const int order = __popc(__ballot_sync(all, may) & below);
   const bool on = may && order < K;
   unsigned same = 0, used = 0;
+  #pragma unroll 4
   for (int j = 0; j < K; ++j) {
     const unsigned those = __ballot_sync(all, on && beam == j);
     if (beam == j) same = those;
@@ -544,21 +545,21 @@ step_kernel(const __grid_constant__ Params p) {
   // ---- the first block: log-sums, scores, the n best
   if (rank == 0) {
     if (warp < K) {
-      float most = -INFINITY;
-      #pragma unroll 1
-      for (int i = row_run > -INFINITY ? lane : S; i < S; i += 32) most = fmaxf(most, sm.umax[warp * S + i]);
-      most = warp_max(most);
+      // a lane's slices first (one, with four beams and eight blocks), then the warp's
+      float mine = -INFINITY, reach = -INFINITY;
       double sum = 0.0;
       #pragma unroll 1
-      for (int i = most > -INFINITY ? lane : S; i < S; i += 32) {
+      for (int i = row_run > -INFINITY ? lane : S; i < S; i += 32) {
         const float um = sm.umax[warp * S + i];
-        if (um == most) sum += sm.usum[warp * S + i];
-        else if (most < INFINITY && um > -INFINITY) sum += sm.usum[warp * S + i] * (double)fast_exp2((um - most) * kLog2e);
+        const double us = sm.usum[warp * S + i];
+        reach = fmaxf(reach, sm.reached[warp * S + i]);
+        if (um > mine) { sum = us + (mine > -INFINITY && um < INFINITY ? sum * (double)fast_exp2((mine - um) * kLog2e) : 0.0); mine = um; }
+        else if (um == mine) sum += um > -INFINITY ? us : 0.0;
+        else if (um > -INFINITY && mine < INFINITY) sum += us * (double)fast_exp2((um - mine) * kLog2e);
       }
-      float reach = -INFINITY;
-      #pragma unroll 1
-      for (int i = most > -INFINITY ? lane : S; i < S; i += 32) reach = fmaxf(reach, sm.reached[warp * S + i]);
+      const float most = warp_max(mine);
       reach = warp_max(reach);
+      if (mine < most) sum = mine > -INFINITY && most < INFINITY ? sum * (double)fast_exp2((mine - most) * kLog2e) : 0.0;
       sum = log_of(warp_sum(sum));
       if (lane == 0) {
         const Row r{row_run, (double)most + sum, sum, !(most > -INFINITY) ? 1 : most == INFINITY ? 2 : 0};
