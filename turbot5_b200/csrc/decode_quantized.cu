@@ -457,20 +457,36 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
   cluster.sync();                        // nobody leaves while its shared memory is read
 }
 
+// What the current device says of a kernel, asked once: the largest cluster and how many blocks are resident at a time.
+template <typename T, int D, int TILES, int WARPS>
+struct Fit {
+  int cluster = 0, resident = 0;
+  static const Fit* get() {
+    static std::atomic<const Fit*> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    if (const Fit* f = known[dev]) return f;
+    const auto kernel = decode_quantized_kernel<T, D, TILES, WARPS>;
+    constexpr int smem = WARPS * Ring<D>::WARP_BYTES;
+    int per_sm = 0, sms = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, WARPS * 32, smem) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return nullptr;
+    Fit* f = new Fit;                    // kept for the life of the process (a second thread may find the same again)
+    f->cluster = largest_cluster((const void*)kernel, WARPS * 32, smem);
+    f->resident = per_sm * sms;
+    if (f->cluster == 0) { delete f; return nullptr; }
+    known[dev] = f;
+    return f;
+  }
+};
+
 template <typename T, int D, int TILES, int WARPS>
 static int launch(const Params& p, const BucketSpec& spec, int C, cudaStream_t stream) {
   constexpr int smem = WARPS * Ring<D>::WARP_BYTES;
-  static std::atomic<int> most[64];      // per device: the largest cluster this kernel can have (found twice, it is the same)
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return T5B_ERR_LAUNCH;
-  if (!most[dev]) {
-    const auto kernel = decode_quantized_kernel<T, D, TILES, WARPS>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return T5B_ERR_LAUNCH;
-    const int found = largest_cluster((const void*)kernel, WARPS * 32, smem);
-    if (found == 0) return T5B_ERR_LAUNCH;
-    most[dev] = found;
-  }
-  if (C > most[dev]) C = most[dev];
+  const auto* fit = Fit<T, D, TILES, WARPS>::get();
+  if (!fit) return T5B_ERR_LAUNCH;
+  if (C > fit->cluster) C = fit->cluster;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)C, (unsigned)p.H, (unsigned)(p.B * p.row_groups));
   cfg.blockDim = dim3(WARPS * 32); cfg.stream = stream; cfg.dynamicSmemBytes = smem;
@@ -485,7 +501,8 @@ static int launch(const Params& p, const BucketSpec& spec, int C, cudaStream_t s
 // GPU decide, so the split goes by heads = B * H * groups of rows and by the items of a whole cache (us on B200):
 //   * up to 212 heads: a block of eight warps each, and clusters up to 1700 warps in all as long as a warp keeps four items
 //     (192 heads x 2048 keys: 9.4, with four warps 10.3; 12 x 102400: 36.1 in clusters of 16, 267 without);
-//   * short caches of many heads: two warps (768 x 512: 12.8, with four 14.3);
+//   * short caches of many heads: two warps (768 x 512: 12.8, with four 14.3), and more heads than blocks of four warps are
+//     resident, up to half as many more (512 x 4096 of 128 columns: 96.8, with four 115.7);
 //   * else four warps (1536 x 2048: 66.9, with two 78.8), two blocks per head for long caches of 400 to 1200 heads, where
 //     one block per head leaves the last round of blocks half empty (1024 x 8192: 165.5, with one 170.2).
 template <typename T, int D, int TILES>
@@ -496,8 +513,12 @@ static int launch_split(const Params& p, const BucketSpec& spec, cudaStream_t st
     while (C < MAX_CLUSTER && heads * 16 * C <= 1700 && items >= 64 * C) C *= 2;
     return launch<T, D, TILES, 8>(p, spec, C, stream);
   }
-  if (heads >= 512 && items <= 16) return launch<T, D, TILES, 2>(p, spec, 1, stream);
-  return launch<T, D, TILES, 4>(p, spec, heads > 400 && heads < 1200 && items >= 256 ? 2 : 1, stream);
+  if (heads > 400 && heads < 1200 && items >= 256) return launch<T, D, TILES, 4>(p, spec, 2, stream);
+  const auto* fit = Fit<T, D, TILES, 4>::get();
+  if (!fit) return T5B_ERR_LAUNCH;
+  if ((heads >= 512 && items <= 16) || (heads > fit->resident && 2 * heads <= 3 * fit->resident))
+    return launch<T, D, TILES, 2>(p, spec, 1, stream);
+  return launch<T, D, TILES, 4>(p, spec, 1, stream);
 }
 
 template <typename T, int D>
