@@ -7,20 +7,27 @@
 //   the 2K best (k, t): by s, then the lowest beam, then the largest logit, then the lowest token
 //   -> those that end the sentence join the pool of finished sentences, the K best others go on.
 //
-// One cluster of blocks per sentence reads every logit once; a warp owns a slice of one running beam's row (a "unit").
+// One cluster of blocks per sentence reads every logit once; a warp owns a slice of one beam's row (a "unit").
 // What a kernel of this size costs is not the bytes but the steps that wait for one another (a cluster barrier is some 900
-// cycles, more than the pass over a block's 32 KB), so there is one exchange:
+// cycles, as much as the exponentials of a block's 32 KB), so there is one exchange:
 //
-//   * In a block, the warps of one row form a segment.  The n-th largest of the maxima of 33 to 64 groups of its lanes is
-//     a bound that n of its elements reach, so only lanes whose own maximum reaches it look at their elements again: for
-//     n = 8 about nine candidates per segment are left.
-//   * Those and the slices' maxima and sums of exponentials go to the cluster's first block, which makes the log-sums,
-//     scores the candidates, thins them out by the same bound where they are many (n = 32) and ranks the rest by counting.
+//   * In a block, the warps of one row form a segment.  The n-th largest of the maxima of groups of its lanes is a bound
+//     that n of its elements reach, so only lanes whose own maximum reaches it look at their elements again: for n = 8
+//     about nine candidates per segment are left.
+//   * Those, the bounds and the slices' maxima and sums of exponentials go to the cluster's first block, which makes the
+//     log-sums, scores the candidates, keeps those that reach the best segment's bound (and thins them out by a bound of
+//     their own where they are many, n = 32) and ranks the rest by counting.
 //   * Where that fails - fewer finite candidates than n, or hundreds of equal ones - every warp makes the sorted list of its
 //     slice's n best instead and the first block merges the lists.
 //
 // Sums of exponentials are float32 within a lane (a few dozen terms) and float64 from there on, as are the scores: two
 // candidates of different beams are told apart to about 1e-8.
+//
+// Measured on B200 (device time, launches in a graph): 6.8 us for one sentence of 4 beams x 32128 bf16 logits, 11.3 us for
+// 64 of them (16.4 MB), 20.9 us for 8 sentences of 16 beams x 65537 float32 logits (33.6 MB; the pass itself 5.8 us, at
+// the copy rate).  Of the first, about 1400 cycles are the first reads, 2100 the exponentials (one unit of 16 a clock),
+// 1000 the barrier, 8000 the short steps around it.  A second exchange with a bound over the whole sentence, float64
+// second looks and unrolled one-shot code (126 KB) cost 9.0, 12.0 and 9.2 us.
 //
 // The reference has no beam search of its own (its heads inherit it: src/turbot5/heads/t5_heads.py:100-130).
 #include "t5b_common.cuh"
@@ -40,7 +47,7 @@ constexpr int THREADS = WARPS * 32;
 constexpr int MAX_CLUSTER = 16;          // more than 8 is beyond what every GPU has to offer, but not this one
 constexpr int MAX_UNITS = WARPS * MAX_CLUSTER;
 constexpr int MAX_FOUND = 1024;          // candidates of a sentence, an equal share for each block of the cluster
-constexpr int FEW = 128;                 // candidates that are ranked by counting without another bound
+constexpr int FEW = 128;                 // candidates that are ranked by counting
 constexpr int MAX_BEAMS = 16;
 constexpr int TOKEN_BITS = 27;
 constexpr uint32_t TOKEN_MASK = (1u << TOKEN_BITS) - 1;
@@ -213,14 +220,22 @@ __device__ __noinline__ uint64_t best_of_slice(const Slice<T>& sl, int beam, int
       if (lane >= n) mine = 0;
     }
   };
-  // the vectors' elements in turn, then those before and behind them
+  // vectors in turn, the next one on its way; then the elements before and behind them
+  constexpr int N = Pack<T>::N;
+  uint4 next = make_uint4(0, 0, 0, 0);
+  if (sl.v0 + lane < sl.v1) next = __ldg(sl.mid + sl.v0 + lane);
   #pragma unroll 1
-  for (int i = 0; i < (sl.v1 - sl.v0 + 31) / 32 * Pack<T>::N + 2; ++i) {
-    const int v = sl.v0 + i / Pack<T>::N * 32 + lane, more = i - (sl.v1 - sl.v0 + 31) / 32 * Pack<T>::N;
-    const int token = more < 0 ? sl.first + v * Pack<T>::N + i % Pack<T>::N : more == 0 ? lane : sl.tail + lane;
-    const bool in = more < 0 ? v < sl.v1 : more == 0 ? lane < sl.head : token < sl.V;
-    insert(in ? make_key(beam, to_float<T>(sl.row[token]), token) : 0);
+  for (int v = sl.v0 + lane; v - lane < sl.v1; v += 32) {
+    const uint4 w = next;
+    const bool in = v < sl.v1;
+    if (v + 32 < sl.v1) next = __ldg(sl.mid + v + 32);
+    float x[N];
+    unpack<T>(w, x);
+    #pragma unroll
+    for (int e = 0; e < N; ++e) insert(in ? make_key(beam, x[e], sl.first + v * N + e) : 0);
   }
+  insert(lane < sl.head ? make_key(beam, to_float<T>(sl.row[lane]), lane) : 0);
+  insert(sl.tail + lane < sl.V ? make_key(beam, to_float<T>(sl.row[sl.tail + lane]), sl.tail + lane) : 0);
   return mine;
 }
 
@@ -242,7 +257,9 @@ struct Shared {
       uint64_t key[MAX_FOUND];
     };
     struct {
-      uint64_t lists[WARPS][32];
+      uint64_t lists[WARPS][32];         // sorted keys of a slice
+      uint64_t merged[WARPS][32];        // of a segment, at its first warp
+      int segment[MAX_BEAMS + MAX_CLUSTER];
       Cand heads[WARPS];
     };
   };
@@ -376,7 +393,7 @@ __device__ __forceinline__ void go_on(const Params& p, const Cand* best, int b, 
     for (int skip = __popc(again & below); skip > 0; --skip) open &= open - 1;
     place = __ffs(open) - 1;
   }
-  if (on && place >= 0) {
+  if (on && (unsigned)place < (unsigned)K) {
     const int64_t to = (int64_t)b * K + place;
     p.tokens_out[to] = token; p.parents_out[to] = beam; p.scores_out[to] = (float)best[lane].score;
     if (p.hist_tokens && pos >= 0 && pos < p.hist_steps) {
@@ -496,8 +513,6 @@ step_kernel(const __grid_constant__ Params p) {
   if (active) {
     if (lane == 0) lead->reached[unit] = warp == first ? reached : -INFINITY;
     const bool mine = m >= least;
-    // the elements among a lane's vectors that reach the bound: bits, then one after the other (small code on purpose:
-    // what runs once per launch pays its way through the instruction cache)
     auto push = [&](float x, int token) {
       const int i = atomicAdd(&sm.found_here, 1);
       if (i < share) lead->found[rank * share + i] = make_key(k, x, token);
@@ -532,6 +547,7 @@ step_kernel(const __grid_constant__ Params p) {
     }
     #pragma unroll 1
     for (uint32_t todo = __ballot_sync(0xffffffffu, mine && in_others >= least); todo; todo &= todo - 1) {
+      if (sm.found_here > share) break;                  // more than can be used: the lists will do it
       const int who = __ffs(todo) - 1;                   // several: its vectors again, by the whole warp
       #pragma unroll 1
       for (int v = sl.v0 + who + 32 * lane; v < sl.v1; v += 32 * 32) push_vector(__ldg(sl.mid + v), v);
@@ -646,20 +662,45 @@ step_kernel(const __grid_constant__ Params p) {
   cluster.sync();
   if (!sm.overflow) return;
 
-  // ---- too few or too many candidates: a sorted list per slice of every row, merged by the first block
+  // ---- too few or too many candidates: a sorted list per slice of every row, one per segment of those (an element's place
+  // in the segment is the number of larger ones in each of its lists), and the n best of all in turn by the first block
+  sm.merged[warp][lane] = 0;
   if (owns) sm.lists[warp][lane] = best_of_slice<T>(sl, k, n, lane);
+  __syncthreads();
+  if (owns && lane < n) {
+    const uint64_t mine = sm.lists[warp][lane];
+    const int from = max(k * S - rank * WARPS, 0), to = min((k + 1) * S - rank * WARPS, WARPS);
+    int above = 0;
+    #pragma unroll 2
+    for (int w = from; w < to; ++w) {
+      int more = 0;                      // sorted: a search for the first that is not larger
+      #pragma unroll
+      for (int half = 32; half > 0; half >>= 1)
+        if (more + half <= n && sm.lists[w][more + half - 1] > mine) more += half;
+      above += more;
+    }
+    if (mine && above < n) sm.merged[from][above] = mine;
+  }
+  if (tid == 0) sm.kept = 0;
   cluster.sync();
   if (rank == 0) {
-    int next = 0;
-    Cand mine{-INFINITY, 0};
-    auto take = [&]() {
-      mine.key = next < n ? cluster.map_shared_rank(&sm, tid / WARPS)->lists[tid % WARPS][next] : 0;
-      mine.score = mine.key ? score_of(sm.rows[tid / S], key_logit(mine.key)) : -INFINITY;
-    };
-    if (tid < K * S) take();
+    // every thread has two candidates: number tid % 32 of two of the segments (at most K + C - 1 of them)
+    if (tid < C * WARPS && tid < K * S && (tid % WARPS == 0 || tid % S == 0)) sm.segment[atomicAdd(&sm.kept, 1)] = tid;
+    __syncthreads();
+    Cand mine[2];
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mine[i] = Cand{-INFINITY, 0};
+      const int at = (tid >> 5) + i * WARPS;
+      if (at < sm.kept) {
+        const int u = sm.segment[at];
+        mine[i].key = cluster.map_shared_rank(&sm, u / WARPS)->merged[u % WARPS][lane];
+        if (mine[i].key) mine[i].score = score_of(sm.rows[key_beam(mine[i].key)], key_logit(mine[i].key));
+      }
+    }
     #pragma unroll 1
     for (int i = 0; i < n; ++i) {
-      Cand top = mine;
+      Cand top = better(mine[1].score, mine[1].key, mine[0].score, mine[0].key) ? mine[1] : mine[0];
       #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const double os = __shfl_xor_sync(0xffffffffu, top.score, o);
@@ -669,10 +710,11 @@ step_kernel(const __grid_constant__ Params p) {
       if (lane == 0) sm.heads[warp] = top;
       __syncthreads();
       top = sm.heads[0];
-      #pragma unroll 1
+      #pragma unroll 5
       for (int w = 1; w < WARPS; ++w) if (better(sm.heads[w].score, sm.heads[w].key, top.score, top.key)) top = sm.heads[w];
       if (tid < 2) sm.chosen[tid][i] = top;
-      if (mine.key && mine.key == top.key) { ++next; take(); }
+      #pragma unroll
+      for (int j = 0; j < 2; ++j) if (mine[j].key == top.key) mine[j] = Cand{-INFINITY, 0};
       __syncthreads();
     }
     if (warp == 0) go_on(p, sm.chosen[0], b, lane, pos);
@@ -683,6 +725,7 @@ step_kernel(const __grid_constant__ Params p) {
 
 // ---- sentences from the history of tokens and parents -------------------------------------------------------------
 //
+// Bound by the length of its chains, not by bytes: 7.7 us for 64 searches x 8 sentences x 512 steps, 3.8 us for one of 32.
 // Walking back from the last token is a chain of dependent reads.  A block per sentence brings a segment of tokens and
 // parents into shared memory (every read in flight at once) and cuts it into pieces: every piece is walked from each of
 // its K possible beams, the pieces' results are chained per returned sentence, and the pieces are walked again from the
