@@ -354,3 +354,12 @@ def test_generation_operators_refuse_cpu_tensors():
         t5b.reorder_beam_cache(3, i)
     with pytest.raises(TypeError):
         t5b.beam_search_step(None, s, s, i, i, None, None)
+
+
+def test_cache_positions_near_the_largest_number_are_refused():
+    from turbot5_b200 import _native as nat
+    L = nat.lib()
+    Fill = _c_struct("t5b_cache_quantize_args")
+    full = {n: 16 for n in ("k", "v", "k_cache", "v_cache", "k_scale", "v_scale")}
+    a = Fill(dtype=nat.F16, B=1, H=2, M=4, D=64, capacity=64, start=(1 << 63) - 2, **full)
+    assert L.t5b_cache_quantize(ctypes.cast(ctypes.byref(a), ctypes.c_void_p), None) == 2

@@ -220,3 +220,11 @@ def test_refusals():
         BeamDecoding(model, states, 4, 2, use_cuda_graph=False).sequences()
     with pytest.raises(ValueError, match="decode_step_static"):
         model.decoder.decode_step(torch.zeros((4, 1), dtype=torch.long, device="cuda"), model.decoder.new_cache(states, 4, beams=2))
+
+
+def test_more_refusals_before_any_step():
+    model, states = _model(), _states(2, 12)
+    with pytest.raises(ValueError, match="sentences"):
+        model.beam_search(states, 4, 2, num_return_sequences=0)
+    with pytest.raises(ValueError, match="beams"):
+        model.generate(torch.zeros((1, 4), dtype=torch.long, device="cuda"), num_beams=0)

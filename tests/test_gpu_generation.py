@@ -684,3 +684,100 @@ def test_refusals_on_the_device():
     fill(x[:, :, :0], x[:, :, :0], k, ks, v, vs, 128)
     t5b.reorder_beam_cache([], parents)
     t5b.beam_search_step(logits[:0], *(t[:0] for t in dev), pos)
+
+
+def test_written_tensors_that_overlap_or_have_gradients_are_refused():
+    """Tensors that a call writes overlap one another, or an input that they do not replace: no order of the threads is
+    promised, so there is no right result."""
+    import turbot5_b200 as t5b
+    s = _search(2, 4, 1, 0)
+    scores, pool, steps, beams, done = (s[n].cuda() for n in ("scores", "pool", "steps", "beams", "done"))
+    pos, logits = torch.zeros(1, dtype=torch.long, device="cuda"), torch.zeros((8, 50), device="cuda")
+    step = lambda out, history=None: t5b.beam_search_step(logits, scores, pool, steps, beams, done, pos, out=out, history=history)
+    fresh = lambda: [torch.empty((2, 4), dtype=d, device="cuda") for d in (torch.long, torch.int32, torch.float32, torch.float32, torch.int32, torch.int32)] + [
+        torch.empty(2, dtype=torch.bool, device="cuda")]
+    shifted = torch.zeros(9, device="cuda")
+    hist = torch.zeros((3, 2, 4), dtype=torch.int32, device="cuda")
+    for change in ({2: pool, 3: scores}, {1: steps}, {2: shifted[:8].view(2, 4), 3: shifted[1:].view(2, 4)}, {3: logits.view(-1)[:8].view(2, 4)}):
+        out = fresh()
+        for i, t in change.items():
+            out[i] = t
+        with pytest.raises(ValueError, match="overlap"):
+            step(out)
+    out = fresh()
+    with pytest.raises(ValueError, match="overlap"):
+        step(out, [hist, hist])
+    with pytest.raises(ValueError, match="overlap"):
+        step([out[0], hist[1], *out[2:]], [hist, torch.zeros_like(hist)])
+    out[2].requires_grad_()
+    with pytest.raises(ValueError, match="gradients"):
+        step(out)
+    before = scores._version
+    step([*out[:2], scores, pool, steps, beams, done])
+    assert scores._version == before + 1
+
+    parents = torch.zeros((2, 4), dtype=torch.int32, device="cuda")
+    both = torch.zeros((9, 3, 10, 16), device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        t5b.reorder_beam_cache([both[:8], both[1:]], parents)
+    between = torch.zeros((8, 2, 3, 10, 16), device="cuda")
+    t5b.reorder_beam_cache([between[:, 0], between[:, 1]], parents)         # one between the other's rows
+    with pytest.raises(ValueError, match="gradients"):
+        t5b.reorder_beam_cache([both[:8].clone().requires_grad_()], parents)
+    x = torch.zeros((2, 3, 5, 64), device="cuda", dtype=torch.bfloat16)
+    cache, scale = torch.zeros((3, 3, 128, 64), device="cuda").to(FP8), torch.ones((2, 2, 3, 2), device="cuda")
+    with pytest.raises(ValueError, match="own"):
+        t5b.quantize_into_cache(x, x, cache[:2], scale[0], cache[1:], scale[1])
+    with pytest.raises(ValueError, match="own"):
+        t5b.quantize_into_cache(x, x, cache[:2], scale[0], cache[:2].clone(), scale.view(-1)[6:18].view(2, 3, 2))
+    version = cache._version
+    t5b.quantize_into_cache(x, x, cache[:2], scale[0], cache[:2].clone(), scale[1])
+    assert cache._version == version + 1
+
+
+def test_lengths_of_other_layouts():
+    """Lengths as a column of a larger tensor, or (B, 1)."""
+    import turbot5_b200 as t5b
+    (k, ks), (v, vs) = ([t.cuda() for t in _cache(2, 3, 128, 64, i)] for i in (1, 2))
+    x = torch.randn((2, 3, 5, 64), device="cuda").bfloat16()
+    lens = torch.tensor([[2, 9], [5, 9]], dtype=torch.int32, device="cuda")
+    want = t5b.flash_decoding_quantized_with_fusing_bias(x, k, ks, v, vs, None, seqlens_k=lens[:, 0].contiguous())
+    assert torch.equal(want, t5b.flash_decoding_quantized_with_fusing_bias(x, k, ks, v, vs, None, seqlens_k=lens[:, :1]))
+    a, b = [[t.clone() for t in (k, ks, v, vs)] for _ in range(2)]
+    t5b.quantize_into_cache(x, x, *a, 64, seqlens=lens[:, 0].contiguous())
+    t5b.quantize_into_cache(x, x, *b, 64, seqlens=lens[:, 0])
+    assert all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(a, b))
+
+
+@pytest.mark.parametrize("value", [1 << 40, (1 << 63) - 1, -1, -(1 << 63)])
+def test_quantize_starts_far_outside_the_cache(value):
+    import turbot5_b200 as t5b
+    (k, ks), (v, vs) = ([t.cuda() for t in _cache(2, 3, 128, 64, i)] for i in (1, 2))
+    before = [t.clone() for t in (k, ks, v, vs)]
+    for M in (1, 70):
+        x = torch.ones((2, 3, M, 64), device="cuda", dtype=torch.bfloat16)
+        t5b.quantize_into_cache(x, x, k, ks, v, vs, torch.tensor([value], device="cuda"))
+    torch.cuda.synchronize()
+    assert all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(before, (k, ks, v, vs)))
+
+
+@pytest.mark.parametrize("D", [16, 128])
+def test_attention_over_more_than_2_31_numbers_of_a_head(D):
+    """The first and the last key of a head whose keys fill more than 2^31 bytes; all others are zero and far below."""
+    import turbot5_b200 as t5b
+    N = (1 << 31) // D + 100
+    cap = -(-N // 64) * 64
+    k, v = (torch.zeros((1, 1, cap, D), dtype=torch.uint8, device="cuda") for _ in range(2))
+    scale = torch.ones((1, 1, cap // 64), device="cuda")
+    q = torch.full((1, 1, 1, D), 4.0, dtype=torch.bfloat16, device="cuda")
+    values = torch.randn((2, D), generator=torch.Generator().manual_seed(1)).cuda().to(FP8)
+    for n, i in ((0, 0), (N - 1, 1)):
+        k[0, 0, n] = torch.full((D,), 4.0, device="cuda").to(FP8).view(torch.uint8)
+        v[0, 0, n] = values[i].view(torch.uint8)
+    out = t5b.flash_decoding_quantized_with_fusing_bias(q, k.view(FP8), scale, v.view(FP8), scale, None, sm_scale=1.0, kv_len=N)
+    # weights 1/2 each and exp(-256) for the others; one bf16 rounding, and float32 ones that are far smaller
+    want = values.double().mean(0)
+    assert ((out[0, 0, 0].double() - want).abs() <= want.abs() * 2.0 ** -8 * 1.01 + 1e-30).all()
+    k[0, 0, 0] = 0
+    out = t5b.flash_decoding_quantized_with_fusing_bias(q, k.view(FP8), scale, v.view(FP8), scale, None, sm_scale=1.0, kv_len=N)
+    assert torch.equal(out[0, 0, 0], values[1].to(torch.bfloat16))

@@ -331,7 +331,8 @@ __device__ __forceinline__ void settle(const Params& p, const Cand* best, int b,
   const unsigned joining = __ballot_sync(all, joins), others = __ballot_sync(all, lane < p.n && !ends);
   const float highest = (float)__shfl_sync(all, score, __ffs(others) - 1);           // the first that goes on
   const float old = lane < K && pool.score == pool.score ? pool.score : -INFINITY;
-  const float fresh = joins ? (float)(score * inv_length) : -INFINITY;
+  const float joining_score = (float)(score * inv_length);         // (0 x inf, a penalty beyond all numbers: NaN)
+  const float fresh = joins && joining_score == joining_score ? joining_score : -INFINITY;
   int old_rank = lane, new_rank = 0;
   const float next = __shfl_down_sync(all, old, 1);
   if (joining || __any_sync(all, lane < K - 1 && next > old)) {

@@ -21,9 +21,10 @@
 //
 // A warp works on items of 32 or 64 keys of one block of 64 (so an item has one scale), with its own running maximum and
 // sum and its own ring of stages in shared memory that asynchronous copies fill ahead (registers alone held too little in
-// flight: 206 us instead of 167 for 1.07 GB, 98 % of the measured copy rate).  Warps merge in shared memory, the blocks of a (batch, head) that share a long cache form a cluster and merge through distributed
-// shared memory: no workspace, no counters, no second launch.  The bias is looked up for items within the largest
-// distance of a query only, from a table of the item's distances that the warp makes for itself.
+// flight: 206 us instead of 167 for 1.07 GB, 98 % of the measured copy rate).  Warps merge in shared memory, the blocks
+// of a (batch, head) that share a long cache form a cluster and merge through distributed shared memory: no workspace,
+// no counters, no second launch.  The bias is looked up for items within the largest distance of a query only, from a
+// table of the item's distances that the warp makes for itself.
 //
 // Semantics: the cached step of T5Attention.forward (src/turbot5/model/attentions.py:198,229-234), the merge rule of
 // src/turbot5/ops/flash_decoding.py:47-55, as in decode.cu.
@@ -195,7 +196,7 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
       const int n0 = it * ITEM;
       const int64_t from = (int64_t)n0 * D;
       const uint32_t to = smem_u32(ring + stage * R::BYTES) + lane * 16;
-      const int bytes = (n_end - n0) * D - lane * 16;      // of this lane's first piece on
+      const int bytes = min(n_end - n0, ITEM) * D - lane * 16;      // of this lane's first piece on
       #pragma unroll
       for (int i = 0; i < (ITEM * D + 511) / 512; ++i)
         if (ITEM * D % 512 == 0 || lane * 16 + i * 512 < ITEM * D) {

@@ -28,8 +28,33 @@ void check_plain(const Tensor& t, at::ScalarType dtype, at::IntArrayRef sizes, a
   check_on(t, dev, name);
   TORCH_CHECK_VALUE(t.is_contiguous(), name, " must be contiguous");
 }
-void check_written(const Tensor& t, const char* name) {
+// Tensors that are written in place: they do not overlap themselves, have no part in gradients, and count the change.
+void check_written(const Tensor& t, const char* name, bool grad) {
   TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, name, " is written and must not overlap itself");
+  TORCH_CHECK_VALUE(!(grad && t.requires_grad()), name, " is written in place and must not require gradients");
+}
+void count_change(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+// The bytes from a tensor's first element to its last.
+struct Span {
+  uintptr_t from = 0, to = 0;
+  explicit Span(const Tensor& t) {
+    if (t.numel() == 0) return;
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    from = (uintptr_t)t.data_ptr(); to = from + (uintptr_t)(last + 1) * t.element_size();
+  }
+  bool meets(const Span& o) const { return from < o.to && o.from < to; }
+};
+// `n` lengths on the device
+Tensor lengths_arg(PyObject* o, int64_t n, at::Device dev, const char* name) {
+  const Tensor t = tensor_arg(o);
+  if (!t.defined()) return t;
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " must be int32");
+  TORCH_CHECK_VALUE(t.numel() == n, name, " must have one entry per row, ", n, ", got ", t.numel());
+  check_on(t, dev, name);
+  return t.contiguous();
 }
 int int32_size(int64_t n, const char* name) {
   TORCH_CHECK_VALUE(n >= 0 && n <= INT32_MAX, name, " is too large: ", n);
@@ -66,6 +91,7 @@ PyObject* tuple_of(const std::vector<Tensor>& ts) {
 PyObject* py_beam_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   expect(n, 13);
+  const bool grad = at::GradMode::is_enabled();
   at::AutoGradMode no_grad(false);
   Tensor logits = tensor_arg(a[0]);
   const Tensor scores = tensor_arg(a[1]);
@@ -106,9 +132,6 @@ PyObject* py_beam_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       else check_plain(out[i], types[i], bk, dev, names[i]);
     }
   }
-  for (int i = 0; i < 7; ++i)
-    for (int j = 0; j < i; ++j)
-      TORCH_CHECK_VALUE(B == 0 || out[i].data_ptr() != out[j].data_ptr(), "two of the tensors in out are the same");
   std::vector<Tensor> history;
   int64_t steps = 0;
   if (a[12] != Py_None) {
@@ -117,6 +140,26 @@ PyObject* py_beam_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     steps = history[0].size(0);
     check_plain(history[0], at::kInt, {steps, B, K}, dev, "history[0] (tokens)");
     check_plain(history[1], at::kInt, {steps, B, K}, dev, "history[1] (parents)");
+  }
+  if (a[11] != Py_None || !history.empty()) {
+    // what is written may be the matching input; it overlaps nothing else
+    std::vector<Span> written;
+    for (const Tensor& t : out) written.emplace_back(t);
+    for (const Tensor& t : history) written.emplace_back(t);
+    const Span read[7] = {Span(logits), Span(pos), Span(scores), Span(pool[0]), Span(pool[1]), Span(pool[2]), Span(done)};
+    for (size_t i = 0; i < written.size(); ++i)
+      for (size_t j = 0; j < i; ++j)
+        TORCH_CHECK_VALUE(!written[i].meets(written[j]), "two of the tensors in out and history are the same or overlap");
+    for (size_t i = 0; i < written.size(); ++i) {
+      for (size_t j = 0; j < 7; ++j)
+        TORCH_CHECK_VALUE(!written[i].meets(read[j]) || (i == j && i >= 2 && written[i].from == read[j].from), i < 7 ? names[i] : "history",
+                          " overlaps an input that it does not replace");
+    }
+    for (size_t i = 0; i < written.size(); ++i) {
+      const Tensor& t = i < 7 ? out[i] : history[i - 7];
+      check_written(t, i < 7 ? names[i] : "history", grad);
+      count_change(t);
+    }
   }
   if (logits.dim() != 2) logits = logits.reshape({B * K, V});
   if (logits.stride(1) != 1) logits = logits.contiguous();
@@ -186,7 +229,7 @@ PyObject* py_beam_sequences(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // A group of equal tensors whose rows are reordered together: dims (outer,) rows, heads, then `tail` contiguous dims.
 struct Rows { int64_t outer = 1, outer_stride = 0, row_stride = 0, head_stride = 0; };
-Rows rows_of(const std::vector<Tensor>& ts, int64_t dims, int64_t R, at::Device dev, const char* name) {
+Rows rows_of(const std::vector<Tensor>& ts, int64_t dims, int64_t R, at::Device dev, const char* name, bool grad) {
   Rows r;
   const Tensor& t0 = ts[0];
   TORCH_CHECK_VALUE(t0.defined() && (t0.dim() == dims || t0.dim() == dims + 1), name, " must have ", dims, " or ", dims + 1, " dimensions");
@@ -201,12 +244,15 @@ Rows rows_of(const std::vector<Tensor>& ts, int64_t dims, int64_t R, at::Device 
     TORCH_CHECK_VALUE(t.defined() && t.sizes() == t0.sizes() && t.strides() == t0.strides() && t.scalar_type() == t0.scalar_type(),
                       name, " must be alike in shape, strides and type");
     check_on(t, dev, name);
-    check_written(t, name);
+    check_written(t, name, grad);
   }
-  std::vector<const void*> at;
-  for (const Tensor& t : ts) at.push_back(t.data_ptr());
+  if (t0.numel() == 0) return r;
+  // tensors without gaps overlap where their spans do; others may lie between one another's rows
+  std::vector<uintptr_t> at;
+  for (const Tensor& t : ts) at.push_back((uintptr_t)t.data_ptr());
   std::sort(at.begin(), at.end());
-  TORCH_CHECK_VALUE(t0.numel() == 0 || std::adjacent_find(at.begin(), at.end()) == at.end(), name, ": the same tensor twice");
+  const uintptr_t apart = t0.is_non_overlapping_and_dense() ? (uintptr_t)t0.numel() * es : 1;
+  for (size_t i = 1; i < at.size(); ++i) TORCH_CHECK_VALUE(at[i] - at[i - 1] >= apart, name, ": the same tensor twice, or two that overlap");
   return r;
 }
 
@@ -214,10 +260,11 @@ Rows rows_of(const std::vector<Tensor>& ts, int64_t dims, int64_t R, at::Device 
 PyObject* py_reorder_caches(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   expect(n, 4);
+  const bool grad = at::GradMode::is_enabled();
   at::AutoGradMode no_grad(false);
   const std::vector<Tensor> caches = tensors_of(a[0], "caches must be a sequence of tensors");
   const std::vector<Tensor> scales = tensors_of(a[3], "scales must be a sequence of tensors");
-  const Tensor parents = tensor_arg(a[1]), seqlens = tensor_arg(a[2]);
+  const Tensor parents = tensor_arg(a[1]);
   TORCH_CHECK_TYPE(parents.defined(), "parents must be a tensor");
   require_cuda(parents);
   TORCH_CHECK_VALUE(parents.dim() == 2, "parents must be (batch, num_beams), got ", parents.sizes());
@@ -225,22 +272,24 @@ PyObject* py_reorder_caches(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_VALUE(K >= 1 && K <= kMaxBeams, "between 1 and ", kMaxBeams, " beams, got ", K);
   const at::Device dev = parents.device();
   check_plain(parents, at::kInt, {B, K}, dev, "parents");
-  if (seqlens.defined()) check_plain(seqlens, at::kInt, {R}, dev, "seqlens");
+  const Tensor seqlens = lengths_arg(a[2], R, dev, "seqlens");
   if (caches.empty()) {
     TORCH_CHECK_VALUE(scales.empty(), "scales belong to caches");
     Py_RETURN_NONE;
   }
-  const Rows c = rows_of(caches, 4, R, dev, "caches");
+  const Rows c = rows_of(caches, 4, R, dev, "caches", grad);
   const int64_t H = caches[0].size(-3), cap = caches[0].size(-2);
   Rows s;
   if (!scales.empty()) {
-    s = rows_of(scales, 3, R, dev, "scales");
+    s = rows_of(scales, 3, R, dev, "scales", grad);
     TORCH_CHECK_TYPE(scales[0].scalar_type() == at::kFloat, "scales must be float32");
     TORCH_CHECK_VALUE(scales.size() == caches.size() && scales[0].dim() + 1 == caches[0].dim() && s.outer == c.outer &&
                           scales[0].size(-2) == H && scales[0].size(-1) == (cap + T5B_CACHE_BLOCK - 1) / T5B_CACHE_BLOCK,
                       "scales of shape ", scales[0].sizes(), " do not belong to caches of shape ", caches[0].sizes());
   }
   if (caches[0].numel() == 0) Py_RETURN_NONE;
+  for (const Tensor& t : caches) count_change(t);
+  for (const Tensor& t : scales) count_change(t);
   t5b_cache_reorder_args g;
   g.parents = (const int32_t*)parents.data_ptr(); g.seqlens = (const int32_t*)ptr(seqlens);
   g.cache_stride_outer = c.outer_stride; g.cache_stride_row = c.row_stride; g.cache_stride_head = c.head_stride;
@@ -281,9 +330,10 @@ void check_cache(const Tensor& cache, const Tensor& scale, int64_t B, int64_t H,
 PyObject* py_cache_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   expect(n, 8);
+  const bool grad = at::GradMode::is_enabled();
   at::AutoGradMode no_grad(false);
   Tensor k = tensor_arg(a[0]), v = tensor_arg(a[1]);
-  const Tensor kc = tensor_arg(a[2]), ks = tensor_arg(a[3]), vc = tensor_arg(a[4]), vs = tensor_arg(a[5]), seqlens = tensor_arg(a[7]);
+  const Tensor kc = tensor_arg(a[2]), ks = tensor_arg(a[3]), vc = tensor_arg(a[4]), vs = tensor_arg(a[5]);
   TORCH_CHECK_TYPE(k.defined() && v.defined(), "k and v must be tensors");
   require_cuda(k); require_cuda(v);
   TORCH_CHECK_TYPE(k.scalar_type() == v.scalar_type(), "k and v must share a dtype");
@@ -294,9 +344,12 @@ PyObject* py_cache_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Device dev = k.device();
   check_on(v, dev, "v");
   check_cache(kc, ks, B, H, D, dev, "k_cache"); check_cache(vc, vs, B, H, D, dev, "v_cache");
-  for (const Tensor* t : {&kc, &vc, &ks, &vs}) check_written(*t, "the cache");
+  for (const Tensor* t : {&kc, &vc, &ks, &vs}) check_written(*t, "the cache", grad);
   TORCH_CHECK_VALUE(kc.sizes() == vc.sizes() && kc.strides() == vc.strides() && ks.strides() == vs.strides(), "k_cache and v_cache must be alike in shape and strides");
-  TORCH_CHECK_VALUE(kc.numel() == 0 || (kc.data_ptr() != vc.data_ptr() && ks.data_ptr() != vs.data_ptr()), "keys and values need caches of their own");
+  const auto apart = [](const Tensor& x, const Tensor& y) {       // (tensors with gaps may lie between one another's rows)
+    return x.numel() == 0 || (x.data_ptr() != y.data_ptr() && !(x.is_non_overlapping_and_dense() && Span(x).meets(Span(y))));
+  };
+  TORCH_CHECK_VALUE(apart(kc, vc) && apart(ks, vs), "keys and values need caches of their own");
   const int64_t cap = kc.size(2);
   t5b_cache_quantize_args g;
   g.start_ptr = nullptr; g.start = 0;
@@ -310,7 +363,8 @@ PyObject* py_cache_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     g.start = int_arg(a[6]);
     TORCH_CHECK_VALUE(g.start >= 0 && g.start <= cap && M <= cap - g.start, "tokens ", g.start, " to ", g.start + M, " do not fit in a cache of ", cap);
   }
-  if (seqlens.defined()) check_plain(seqlens, at::kInt, {B}, dev, "seqlens");
+  const Tensor seqlens = lengths_arg(a[7], B, dev, "seqlens");
+  for (const Tensor* t : {&kc, &vc, &ks, &vs}) count_change(*t);
   k = unit_stride_last(k); v = unit_stride_last(v);
   g.k = k.data_ptr(); g.v = v.data_ptr(); g.k_cache = kc.data_ptr(); g.v_cache = vc.data_ptr();
   g.k_scale = (float*)ks.data_ptr(); g.v_scale = (float*)vs.data_ptr();
@@ -332,7 +386,7 @@ PyObject* py_decode_quantized(PyObject*, PyObject* const* a, Py_ssize_t n) {
   expect(n, 13);
   at::AutoGradMode no_grad(false);
   Tensor q = tensor_arg(a[0]), bias = tensor_arg(a[5]);
-  const Tensor k = tensor_arg(a[1]), ks = tensor_arg(a[2]), v = tensor_arg(a[3]), vs = tensor_arg(a[4]), seqlens = tensor_arg(a[11]);
+  const Tensor k = tensor_arg(a[1]), ks = tensor_arg(a[2]), v = tensor_arg(a[3]), vs = tensor_arg(a[4]);
   TORCH_CHECK_TYPE(q.defined(), "q must be a tensor");
   require_cuda(q);
   TORCH_CHECK_TYPE(is_half_type(q.scalar_type()), "queries of an 8-bit cache are float16 or bfloat16, got ", c10::toString(q.scalar_type()));
@@ -345,7 +399,7 @@ PyObject* py_decode_quantized(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_VALUE(v.size(2) == cap, "k and v must have one capacity");
   const int64_t N = opt_int(a[10]).value_or(cap);
   TORCH_CHECK_VALUE(N >= 0 && N <= cap, "kv_len exceeds the cache capacity");
-  if (seqlens.defined()) check_plain(seqlens, at::kInt, {B}, dev, "seqlens_k");
+  const Tensor seqlens = lengths_arg(a[11], B, dev, "seqlens_k");
   t5b_decode_quantized_args g;
   g.num_buckets = int32_option(int_arg(a[8]), "NUM_BUCKETS"); g.max_distance = int32_option(int_arg(a[9]), "MAX_DISTANCE");
   g.table = nullptr; g.table_dtype = T5B_F32; g.table_stride0 = 0;

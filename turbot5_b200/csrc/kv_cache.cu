@@ -117,8 +117,8 @@ __device__ __forceinline__ uint2 rescale8(uint2 v, float f) {
 // A team of TEAM threads fills one block of 64 tokens of one head, keys or values.  TEAM 128 for prompts: every thread
 // holds its share of the block between the search for the largest and the rounding (one read of the source), as packed
 // as it came: magnitudes are compared as whole numbers, two at a time, which leaves 3.5 instructions per element (12 with
-// floats throughout): 11.2 us for 53 MB instead of 22.8, and 805 MB at the measured copy rate (119 us).  TEAM 32 for single tokens: a warp has one row to write, four heads
-// share a block of threads.
+// floats throughout): 11.2 us for 53 MB instead of 22.8, and 805 MB at the measured copy rate (119 us).  TEAM 32 for
+// single tokens: a warp has one row to write, four heads share a block of threads.
 template <typename T, int D, int TEAM>
 __global__ void __launch_bounds__(128)
 fill_kernel(const __grid_constant__ FillParams p) {
@@ -132,10 +132,11 @@ fill_kernel(const __grid_constant__ FillParams p) {
   if (TEAM == 32 && head >= p.H) return;                           // whole warps
   const int64_t start = p.start_ptr ? *p.start_ptr : p.start;
   const int count = p.seqlens ? min(max(p.seqlens[b], 0), p.M) : p.M;
+  if (start < 0 || start >= p.cap) return;
   const int64_t end = min(start + (int64_t)count, (int64_t)p.cap);
   const int64_t first = (start / BLOCK + blockIdx.y) * BLOCK;      // the block's first token
   const int64_t begin = first > start ? first : start;
-  if (start < 0 || begin >= end) return;                           // the same for the whole team
+  if (begin >= end) return;                                        // the same for the whole team
   // within the block, the written tokens are [lo, hi)
   const int lo = (int)(begin - first), hi = (int)min(end - first, (int64_t)BLOCK);
   const int token = (TEAM == 32 ? lo : 0) + lane / PARTS, part = lane % PARTS * 8;
@@ -331,7 +332,7 @@ extern "C" int t5b_cache_quantize(const t5b_cache_quantize_args* a, void* stream
   if (!a->start_ptr && a->start < 0) return T5B_ERR_ARG;
   if (a->B == 0 || a->H == 0 || a->M == 0) return T5B_OK;
   if (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale) return T5B_ERR_ARG;
-  if (!a->start_ptr && a->start + a->M > a->capacity) return T5B_ERR_SHAPE;
+  if (!a->start_ptr && a->start > (int64_t)a->capacity - a->M) return T5B_ERR_SHAPE;
   const int es = dtype_bytes(a->dtype);
   kvcache::FillParams p;
   p.src[0] = a->k; p.src[1] = a->v;

@@ -34,8 +34,8 @@ def beam_search_step(logits, scores, finished_scores, finished_steps, finished_b
     (pos + 1) ** length_penalty is above the pool's worst, or when nothing can go on (all running scores -inf).  From then
     on its scores and pool stay, its tokens are `pad_token_id` and its parents itself.
 
-    `pos` is the step's number from 0, one int64 on the device.  `out`: seven tensors to write to, among them the inputs
-    if wanted.  `history`: two int32 (steps, batch, num_beams) tensors whose row `pos` gets tokens and parents.
+    `pos` is the step's number from 0, one int64 on the device.  `out`: seven tensors to write to, each of them the
+    matching input if wanted.  `history`: two int32 (steps, batch, num_beams) tensors whose row `pos` gets tokens and parents.
     NaN logits count as -inf; where a row has +inf, those tokens share the whole probability.  num_beams is at most 16."""
     return _host.beam_step(logits, scores, finished_scores, finished_steps, finished_beams, done, pos, eos_token_id,
                            pad_token_id, length_penalty, early_stopping, out, history)

@@ -558,8 +558,8 @@ class T5Stack(nn.Module):
     # ---- generation with a preallocated cache (decoder only)
     def new_cache(self, encoder_hidden_states, max_len, beams=1, cache_dtype=None, encoder_seqlens=None) -> DecoderCache:
         """A cache for `max_len` steps over these encoder states, in the model's type or (`cache_dtype`
-        torch.float8_e4m3fn) in 8 bits; `beams` rows of self-attention per sentence.  `encoder_seqlens`: only so many
-        states of each sentence count for the scales of an 8-bit cache."""
+        torch.float8_e4m3fn) in 8 bits; `beams` rows of self-attention per sentence.  `encoder_seqlens`: an 8-bit cache
+        keeps only so many states of each sentence (a step that attends has to have these lengths or shorter ones)."""
         cfg = self.cfg
         B = encoder_hidden_states.shape[0]
         cache = _cache_class(cache_dtype)(len(self.block), B, cfg.num_heads, cfg.d_kv, max_len, encoder_hidden_states.dtype,
@@ -826,14 +826,15 @@ class BeamDecoding:
         self.graph = None
         self.rewind()
         if use_cuda_graph:
-            side = torch.cuda.Stream(dev)
-            side.wait_stream(torch.cuda.current_stream(dev))
-            with torch.cuda.stream(side), torch.no_grad():
-                self._step()                             # library handles and stacked weights exist from here on
-            torch.cuda.current_stream(dev).wait_stream(side)
-            self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph), torch.no_grad():
-                self._step()
+            with torch.cuda.device(dev):
+                side = torch.cuda.Stream(dev)
+                side.wait_stream(torch.cuda.current_stream(dev))
+                with torch.cuda.stream(side), torch.no_grad():
+                    self._step()                         # library handles and stacked weights exist from here on
+                torch.cuda.current_stream(dev).wait_stream(side)
+                self.graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(self.graph), torch.no_grad():
+                    self._step()
             self.rewind()
 
     def rewind(self):
@@ -987,6 +988,8 @@ class T5ForConditionalGeneration(nn.Module):
         search (`beam_search`, which takes the options after it).  `cache_dtype` torch.float8_e4m3fn keeps keys and values
         in 8 bits.  Returns the generated ids (B, max_new_tokens); (B, num_return_sequences, max_new_tokens) with more than
         one sentence."""
+        if num_beams < 1:
+            raise ValueError("between 1 and %d beams, got %d" % (MAX_BEAMS, num_beams))
         if num_beams == 1 and num_return_sequences != 1:
             raise ValueError("greedy generation has one sentence to return")
         fused = self.cfg.attention_type == "flash" and input_ids.is_cuda and \
@@ -1014,6 +1017,8 @@ class T5ForConditionalGeneration(nn.Module):
         (B, num_return_sequences)), best first, `pad_token_id` behind the end of a sentence.  A sentence's score is its
         log-probability over its length to the power of `length_penalty`; `early_stopping` ends a search as soon as
         num_beams sentences are finished.  Whether all searches have ended is looked up every 16 steps."""
+        if not 1 <= num_return_sequences <= num_beams:
+            raise ValueError("between 1 and num_beams = %d sentences, got %d" % (num_beams, num_return_sequences))
         search = BeamDecoding(self, encoder_hidden_states, steps, num_beams, encoder_seqlens, length_penalty, early_stopping,
                               cache_dtype, use_cuda_graph)
         for t in range(steps):
