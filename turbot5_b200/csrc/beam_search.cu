@@ -44,7 +44,6 @@ namespace beam {
 
 constexpr int WARPS = 16;
 constexpr int THREADS = WARPS * 32;
-constexpr int MAX_CLUSTER = 16;          // more than 8 is beyond what every GPU has to offer, but not this one
 constexpr int MAX_UNITS = WARPS * MAX_CLUSTER;
 constexpr int MAX_FOUND = 1024;          // candidates of a sentence, an equal share for each block of the cluster
 constexpr int FEW = 128;                 // candidates that are ranked by counting
@@ -873,28 +872,38 @@ sequences_kernel(const __grid_constant__ SequenceParams p) {
   }
 }
 
-static int cluster_blocks(int B, int K, int64_t bytes, int most) {
-  // Two blocks per multiprocessor keep the whole batch resident; more blocks per sentence shorten its pass, 16 only where
-  // a slice would not fit a warp's registers with 8 (a sentence of 4 x 32128 16-bit logits: 7.9 us with 8, 8.5 with 16;
-  // of 16 x 65537 float32: 26.7 and 21.6).  A beam has two warps at least, for the number of groups that its bound is
-  // taken from.
-  int C = bytes > 8 * WARPS * 32 * 4 * 16 ? most : 8;
-  while (C > (K > 8 ? 2 : 1) && (long long)B * C > (C == 16 ? 148 : 2 * 148)) C /= 2;
-  return C;
+// What the current device says of a kernel, asked once.
+template <typename T>
+struct Fit {
+  int clusters[5];                       // resident clusters of 1, 2, 4, 8, 16 blocks
+  static const Fit* get() {
+    static std::atomic<const Fit*> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    if (const Fit* f = known[dev]) return f;
+    Fit* f = new Fit;                    // kept for the life of the process (a second thread may find the same again)
+    if (!resident_clusters((const void*)step_kernel<T>, THREADS, 0, f->clusters)) { delete f; return nullptr; }
+    known[dev] = f;
+    return f;
+  }
+};
+
+static int cluster_log2(int B, int K, int64_t bytes, const int (&clusters)[5]) {
+  // The whole batch is resident; more blocks per sentence shorten its pass, 16 only where a slice would not fit a warp's
+  // registers with 8 (a sentence of 4 x 32128 16-bit logits: 7.9 us with 8, 8.5 with 16; of 16 x 65537 float32: 26.7 and
+  // 21.6) and half of the blocks' places are enough.  A beam has two warps at least, for the number of groups that its
+  // bound is taken from.
+  int c = bytes > 8 * WARPS * 32 * 4 * 16 ? 4 : 3;
+  while (c > (K > 8 ? 1 : 0) && B > (c == 4 ? clusters[4] / 2 : clusters[c])) --c;
+  return c;
 }
 
 template <typename T>
 static int launch_step(Params p, cudaStream_t stream) {
-  static std::atomic<int> most[64];      // per device: the largest cluster this kernel can have (found twice, it is the same)
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return T5B_ERR_LAUNCH;
-  if (!most[dev]) {
-    const int found = largest_cluster((const void*)step_kernel<T>, THREADS, 0);
-    if (found == 0) return T5B_ERR_LAUNCH;
-    most[dev] = found;
-  }
-  const int C = cluster_blocks(p.B, p.K, (int64_t)p.K * p.V * sizeof(T), most[dev]);
-  for (p.cluster_log2 = 0; 1 << p.cluster_log2 < C;) ++p.cluster_log2;
+  const auto* fit = Fit<T>::get();
+  if (!fit) return T5B_ERR_LAUNCH;
+  p.cluster_log2 = cluster_log2(p.B, p.K, (int64_t)p.K * p.V * sizeof(T), fit->clusters);
+  const int C = 1 << p.cluster_log2;
   p.S = C * WARPS / p.K;
   p.unit_magic = (65536u + p.S - 1) / p.S; p.slice_magic = (uint32_t)(((1ull << 32) + p.S - 1) / p.S);
   cudaLaunchConfig_t cfg = {};

@@ -40,7 +40,6 @@ namespace t5b {
 namespace decq {
 
 constexpr int BLOCK = T5B_CACHE_BLOCK;
-constexpr int MAX_CLUSTER = 16;          // more than 8 is beyond what every GPU has to offer, but not this one
 // 16-key tiles of an item, and how its stages lie in shared memory: keys, values, two scales
 template <int D> struct Ring {
   static constexpr int SUB = D == 128 ? 2 : D == 64 ? 2 : 4;
@@ -459,10 +458,10 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
   cluster.sync();                        // nobody leaves while its shared memory is read
 }
 
-// What the current device says of a kernel, asked once: the largest cluster and how many blocks are resident at a time.
+// What the current device says of a kernel, asked once: how many blocks, and clusters of 1, 2, 4, 8 and 16, are resident.
 template <typename T, int D, int TILES, int WARPS>
 struct Fit {
-  int cluster = 0, resident = 0;
+  int resident = 0, clusters[5];
   static const Fit* get() {
     static std::atomic<const Fit*> known[64];
     int dev = 0;
@@ -475,9 +474,8 @@ struct Fit {
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, WARPS * 32, smem) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return nullptr;
     Fit* f = new Fit;                    // kept for the life of the process (a second thread may find the same again)
-    f->cluster = largest_cluster((const void*)kernel, WARPS * 32, smem);
     f->resident = per_sm * sms;
-    if (f->cluster == 0) { delete f; return nullptr; }
+    if (!resident_clusters((const void*)kernel, WARPS * 32, smem, f->clusters)) { delete f; return nullptr; }
     known[dev] = f;
     return f;
   }
@@ -486,9 +484,7 @@ struct Fit {
 template <typename T, int D, int TILES, int WARPS>
 static int launch(const Params& p, const BucketSpec& spec, int C, cudaStream_t stream) {
   constexpr int smem = WARPS * Ring<D>::WARP_BYTES;
-  const auto* fit = Fit<T, D, TILES, WARPS>::get();
-  if (!fit) return T5B_ERR_LAUNCH;
-  if (C > fit->cluster) C = fit->cluster;
+  if (!Fit<T, D, TILES, WARPS>::get()) return T5B_ERR_LAUNCH;            // (which allows the launch that much shared memory)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)C, (unsigned)p.H, (unsigned)(p.B * p.row_groups));
   cfg.blockDim = dim3(WARPS * 32); cfg.stream = stream; cfg.dynamicSmemBytes = smem;
@@ -501,8 +497,10 @@ static int launch(const Params& p, const BucketSpec& spec, int C, cudaStream_t s
 
 // Warps per head.  What a block costs beyond its keys (lengths, queries, bias, two merges) and how the last blocks fill the
 // GPU decide, so the split goes by heads = B * H * groups of rows and by the items of a whole cache (us on B200):
-//   * up to 212 heads: a block of eight warps each, and clusters up to 1700 warps in all as long as a warp keeps four items
-//     (192 heads x 2048 keys: 9.4, with four warps 10.3; 12 x 102400: 36.1 in clusters of 16, 267 without);
+//   * up to 212 heads, if all of their blocks are resident at a time: a block of eight warps each (192 heads x 2048 keys:
+//     9.4, with four warps 10.3; 160 x 1024 of 128 columns, where one such block fits: 19.9 and 16.4), and clusters up to
+//     1700 warps in all as long as a warp keeps four items and all are resident (12 x 102400: 36.1 in clusters of 16, 267
+//     without; 24 x 9664 of 128 columns, 5 rows: 23.3 in clusters of 4, 29.7 of 8, which are not);
 //   * short caches of many heads: two warps (768 x 512: 12.8, with four 14.3), and more heads than blocks of four warps are
 //     resident, up to half as many more (512 x 4096 of 128 columns: 96.8, with four 115.7);
 //   * else four warps (1536 x 2048: 66.9, with two 78.8), two blocks per head for long caches of 400 to 1200 heads, where
@@ -511,9 +509,13 @@ template <typename T, int D, int TILES>
 static int launch_split(const Params& p, const BucketSpec& spec, cudaStream_t stream) {
   const int64_t heads = (int64_t)p.B * p.H * p.row_groups, items = (p.N + Ring<D>::ITEM - 1) / Ring<D>::ITEM;
   if (heads <= 212 && items >= 16) {
-    int C = 1;
-    while (C < MAX_CLUSTER && heads * 16 * C <= 1700 && items >= 64 * C) C *= 2;
-    return launch<T, D, TILES, 8>(p, spec, C, stream);
+    const auto* fit = Fit<T, D, TILES, 8>::get();
+    if (!fit) return T5B_ERR_LAUNCH;
+    if (heads <= fit->resident) {
+      int c = 0;
+      while (c < 4 && heads * (16 << c) <= 1700 && items >= 64 << c && heads <= fit->clusters[c + 1]) ++c;
+      return launch<T, D, TILES, 8>(p, spec, 1 << c, stream);
+    }
   }
   if (heads > 400 && heads < 1200 && items >= 256) return launch<T, D, TILES, 4>(p, spec, 2, stream);
   const auto* fit = Fit<T, D, TILES, 4>::get();

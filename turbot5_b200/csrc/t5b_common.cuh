@@ -69,19 +69,27 @@ __device__ __forceinline__ float load_table(const void* table, int dtype, int64_
   return __bfloat162float(((const __nv_bfloat16*)table)[idx]);
 }
 
-// Blocks per cluster that this kernel can be launched with on the current device: 16 where the GPU has room for such a
-// cluster (beyond the portable size), else 8; 0 after an error.
-inline int largest_cluster(const void* kernel, int threads, int dynamic_smem) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return 0;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(16); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = (size_t)dynamic_smem;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 16; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr; cfg.numAttrs = 1;
-  int clusters = 0;
-  if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) { cudaGetLastError(); return 8; }
-  return clusters > 0 ? 16 : 8;
+// Clusters of 1, 2, 4, 8 and 16 blocks of this kernel that the current device holds at a time (a cluster stays within one
+// part of the GPU, so these are fewer than the blocks would give).  The largest size is beyond the portable one: 0 where
+// the GPU has no room for it.  False after an error.
+constexpr int MAX_CLUSTER = 16;
+inline bool resident_clusters(const void* kernel, int threads, int dynamic_smem, int (&clusters)[5]) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+  for (int i = 0; i < 5; ++i) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1u << i); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = (size_t)dynamic_smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << i; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    clusters[i] = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters[i], kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      if (i < 4) return false;
+      clusters[i] = 0;
+    }
+  }
+  return true;
 }
 
 __host__ __device__ __forceinline__ int dtype_bytes(int dtype) { return dtype == T5B_F32 ? 4 : 2; }
