@@ -201,10 +201,17 @@ fill_kernel(const __grid_constant__ FillParams p) {
 // Bound by the bytes of the beams that change.  A thread owns offsets of all beams of a sentence: it loads what the
 // changed beams are to become, then stores it, so the caches are permuted in place without a second copy and without
 // ordering between threads, whatever the parents are.  Beams that stay are neither read nor written, nor is what lies
-// behind the tokens in use; all layers are one launch.  Four offsets at a time with four beams (two with eight) keep 85
-// registers and 24 warps: 95.7 us for 590 MB, 94 % of the measured copy rate (one offset at a time 114, four with only
-// two blocks per multiprocessor 108).
-constexpr int REORDER_THREADS = 256;
+// behind the tokens in use; all layers are one launch.  Two offsets at a time with four beams keep 64 registers and 32
+// warps: 96.0 us for 590 MB, 94 % of the measured copy rate (one offset at a time 114, four with two blocks per
+// multiprocessor 104, four with three spill in the loop: 120).
+//
+// How much of a cache is in use is known on the device only, so the grid is made for its capacity and a block that finds
+// nothing costs as much as one that moves 16 KB: heads share a few hundred blocks, each of which takes piece after piece,
+// and short heads get blocks of 64 threads.  16 beams of 104 of 470 tokens (92 MB): 24 us, 77 with a block per piece; 3
+// beams of 37 of 229 tokens in 24 layers (65 MB): 19 and 40.
+constexpr int REORDER_THREADS = 2 * 148 * 256;             // beyond these a block takes several pieces of a head
+
+constexpr int in_flight(int beams) { return beams == 16 ? 1 : 2; }
 
 struct ReorderGroup {
   void* base[T5B_REORDER_MAX_TENSORS];
@@ -218,12 +225,12 @@ struct ReorderParams {
 };
 
 // One offset of all beams at a time, UN of them in flight: `at(i)` is the i-th offset's address in the first beam.
-template <typename U, int KM, int UN, typename F>
+template <typename U, int KM, int UN, int THREADS, typename F>
 __device__ __forceinline__ void move_beams(int first, int total, int64_t row_b, const int (&parent)[KM], uint32_t changed, F at) {
   U v[UN][KM];
   #pragma unroll
   for (int u = 0; u < UN; ++u) {
-    const int i = first + u * REORDER_THREADS;
+    const int i = first + u * THREADS;
     if (i < total) {
       const char* from = at(i);
       #pragma unroll
@@ -233,7 +240,7 @@ __device__ __forceinline__ void move_beams(int first, int total, int64_t row_b, 
   }
   #pragma unroll
   for (int u = 0; u < UN; ++u) {
-    const int i = first + u * REORDER_THREADS;
+    const int i = first + u * THREADS;
     if (i < total) {
       char* to = at(i);
       #pragma unroll
@@ -243,12 +250,12 @@ __device__ __forceinline__ void move_beams(int first, int total, int64_t row_b, 
   }
 }
 
-// A block has REORDER_THREADS * UN units of one head's tokens, or all scales of one tensor (blocks behind those of the
-// caches).
-template <typename U, int KM>
-__global__ void __launch_bounds__(REORDER_THREADS, KM <= 8 ? 3 : 2)
+// A block has UN units a thread of one head's tokens, or some times as many, or all scales of one tensor (blocks behind
+// those of the caches).
+template <typename U, int KM, int THREADS>
+__global__ void __launch_bounds__(THREADS, (KM == 4 ? 4 : KM == 8 ? 3 : 2) * 256 / THREADS)
 reorder_kernel(const __grid_constant__ ReorderParams p) {
-  constexpr int UN = 16 / KM;
+  constexpr int UN = in_flight(KM);
   const int b = blockIdx.y, K = p.K, tid = threadIdx.x;
   int parent[KM], len = 0;
   uint32_t changed = 0;
@@ -268,32 +275,44 @@ reorder_kernel(const __grid_constant__ ReorderParams p) {
     const ReorderGroup& g = p.g[0];
     const int chunk = blockIdx.x % p.chunks, rest = blockIdx.x / p.chunks, h = rest % p.H, z = rest / p.H;
     char* base = (char*)g.base[z / g.outer] + (int64_t)(z % g.outer) * g.outer_b + (int64_t)b * K * g.row_b + (int64_t)h * g.head_b;
-    move_beams<U, KM, UN>(chunk * REORDER_THREADS * UN + tid, len * p.units, g.row_b, parent, changed,
-                          [&](int i) { return base + (int64_t)i * sizeof(U); });
+    const int total = len * p.units;
+    #pragma unroll 1
+    for (int i = chunk * THREADS * UN + tid; i < total; i += p.chunks * THREADS * UN)
+      move_beams<U, KM, UN, THREADS>(i, total, g.row_b, parent, changed, [&](int k) { return base + (int64_t)k * sizeof(U); });
   } else {
     const ReorderGroup& g = p.g[1];
     const int z = blockIdx.x - blocks, per_head = (len + BLOCK - 1) / BLOCK, total = per_head * p.H;
     char* base = (char*)g.base[z / g.outer] + (int64_t)(z % g.outer) * g.outer_b + (int64_t)b * K * g.row_b;
-    for (int i = tid; i < total; i += REORDER_THREADS * UN)
-      move_beams<uint32_t, KM, UN>(i, total, g.row_b, parent, changed, [&](int k) {
+    for (int i = tid; i < total; i += THREADS * UN)
+      move_beams<uint32_t, KM, UN, THREADS>(i, total, g.row_b, parent, changed, [&](int k) {
         const int h = k / per_head;
         return base + (int64_t)h * g.head_b + (int64_t)(k - h * per_head) * 4;
       });
   }
 }
 
-template <typename U>
+template <typename U, int KM, int THREADS>
 static int launch_reorder(ReorderParams& p, int B, cudaStream_t stream) {
-  const int un = p.K <= 4 ? 4 : p.K <= 8 ? 2 : 1;
+  constexpr int CHUNK = THREADS * in_flight(KM);
   const int64_t units = (int64_t)p.cap * p.units;
-  p.chunks = (int)((units + REORDER_THREADS * un - 1) / (REORDER_THREADS * un));
-  const int64_t blocks = (int64_t)p.g[0].n * p.g[0].outer * p.H * p.chunks + (int64_t)p.g[1].n * p.g[1].outer;
-  if (blocks > 0x7fffffffll || units > 0x7fffffffll - REORDER_THREADS * 4) return T5B_ERR_SHAPE;
-  const dim3 grid((unsigned)blocks, (unsigned)B);
-  if (p.K <= 4) reorder_kernel<U, 4><<<grid, REORDER_THREADS, 0, stream>>>(p);
-  else if (p.K <= 8) reorder_kernel<U, 8><<<grid, REORDER_THREADS, 0, stream>>>(p);
-  else reorder_kernel<U, 16><<<grid, REORDER_THREADS, 0, stream>>>(p);
+  if constexpr (THREADS > 64)
+    if (units <= CHUNK / 2) return launch_reorder<U, KM, 64>(p, B, stream);
+  // as many blocks as the whole capacity needs, but not more than some rounds of them: the tokens in use are known on the
+  // device only
+  const int64_t heads = (int64_t)p.g[0].n * p.g[0].outer * p.H, most = REORDER_THREADS / THREADS / (heads * B);
+  const int64_t chunks = (units + CHUNK - 1) / CHUNK;
+  p.chunks = (int)(most < 1 ? 1 : chunks < most ? chunks : most);
+  const int64_t blocks = heads * p.chunks + (int64_t)p.g[1].n * p.g[1].outer;
+  if (blocks > 0x7fffffffll || units > 0x7fffffffll - (1 << 24)) return T5B_ERR_SHAPE;
+  reorder_kernel<U, KM, THREADS><<<dim3((unsigned)blocks, (unsigned)B), THREADS, 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? T5B_OK : T5B_ERR_LAUNCH;
+}
+
+template <typename U>
+static int launch_reorder_beams(ReorderParams& p, int B, cudaStream_t stream) {
+  if (p.K <= 4) return launch_reorder<U, 4, 256>(p, B, stream);
+  if (p.K <= 8) return launch_reorder<U, 8, 256>(p, B, stream);
+  return launch_reorder<U, 16, 256>(p, B, stream);
 }
 
 template <typename T, int D>
@@ -389,7 +408,7 @@ extern "C" int t5b_beam_cache_reorder(const t5b_cache_reorder_args* a, void* str
   p.parents = a->parents; p.seqlens = a->seqlens;
   p.K = a->num_beams; p.H = a->H; p.cap = a->capacity; p.units = a->token_bytes / unit;
   cudaStream_t st = (cudaStream_t)stream;
-  if (unit == 16) return kvcache::launch_reorder<uint4>(p, a->B, st);
-  if (unit == 4) return kvcache::launch_reorder<uint32_t>(p, a->B, st);
-  return kvcache::launch_reorder<uint8_t>(p, a->B, st);
+  if (unit == 16) return kvcache::launch_reorder_beams<uint4>(p, a->B, st);
+  if (unit == 4) return kvcache::launch_reorder_beams<uint32_t>(p, a->B, st);
+  return kvcache::launch_reorder_beams<uint8_t>(p, a->B, st);
 }
