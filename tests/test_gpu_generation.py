@@ -781,3 +781,23 @@ def test_attention_over_more_than_2_31_numbers_of_a_head(D):
     k[0, 0, 0] = 0
     out = t5b.flash_decoding_quantized_with_fusing_bias(q, k.view(FP8), scale, v.view(FP8), scale, None, sm_scale=1.0, kv_len=N)
     assert torch.equal(out[0, 0, 0], values[1].to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,K,V", [(3, 4, 384), (2, 10, 384), (1, 16, 384), (40, 10, 126), (1, 1, 15), (2, 8, 65), (1, 4, 4097), (1, 4, 4300), (9, 5, 1000)])
+def test_step_of_small_vocabularies(B, K, V, dtype):
+    """Slices of a few vectors, whose elements the lanes share, with rows that start anywhere and masked and special numbers."""
+    for offset, special in ((0, False), (3, True)):
+        x = _logits(B, K, V, torch.float32, 41 + offset)
+        if special:
+            x[0, ::3] = NONE
+            x[-1, 1::5] = float("nan")
+        x = x.to(dtype)
+        flat = torch.zeros(offset + B * K * (V + offset), dtype=dtype)
+        rows = flat[offset:].view(B * K, V + offset)[:, :V] if offset else x
+        if offset:
+            rows.copy_(x)
+            flat = flat.cuda()
+            rows = flat[offset:].view(B * K, V + offset)[:, :V]
+        s = _search(B, K, 42, 3)
+        _check_step(_run_step(rows if offset else rows.cuda(), s), x, s)

@@ -147,6 +147,17 @@ template <typename T, int U> __device__ __forceinline__ uint32_t mask_of(const u
   }
   return mask;
 }
+// One of a vector's 2^sub equal parts, -inf in place of the others.
+template <typename T> __device__ __forceinline__ uint4 part_of(const uint4& u, int sub, int part) {
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  #pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if ((sub < 3 ? j >> (2 - sub) : 2 * j + (part & 1)) != part) w[j] = Pack<T>::none;
+    else if (sub == 3) w[j] = part & 1 ? (w[j] & 0xffff0000u) | (Pack<T>::none & 0xffffu) : (w[j] & 0xffffu) | (Pack<T>::none & 0xffff0000u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <typename T> struct Lowest;     // the lowest finite number: the bound of what can be chosen
 template <> struct Lowest<float> { static constexpr float value = -3.402823466e38f; };
 template <> struct Lowest<__half> { static constexpr float value = -65504.f; };
@@ -403,7 +414,9 @@ __device__ __forceinline__ void go_on(const Params& p, const Cand* best, int b, 
   }
 }
 
-template <typename T>
+// SHORT: slices of at most 16 vectors, each of which 2^sub lanes share, so that a segment's bound has groups enough to be
+// taken from (small vocabularies: 10 beams x 384 bf16 8.2 us, 39 by the lists without it; 5 x 1000 8.2 and 37).
+template <typename T, bool SHORT>
 __global__ void __launch_bounds__(THREADS, 2)
 step_kernel(const __grid_constant__ Params p) {
   __shared__ Shared sm;
@@ -419,13 +432,15 @@ step_kernel(const __grid_constant__ Params p) {
   const bool owns = row < K;
   const int k = owns ? row : 0;
   const Slice<T> sl((const T*)p.logits + (at + k) * p.row_stride, p.V, owns ? unit - row * S : 0, S, p.slice_magic);
-  constexpr int N = Pack<T>::N, U = 4;
+  constexpr int N = Pack<T>::N, U = SHORT ? 1 : 4;
+  const int span = sl.v1 - sl.v0, sub = !SHORT ? 0 : span > 8 ? 1 : span > 4 || N == 4 ? 2 : 3, of = lane >> sub;
   uint4 u[U];
   #pragma unroll
   for (int i = 0; i < U; ++i) {
     u[i] = make_uint4(Pack<T>::none, Pack<T>::none, Pack<T>::none, Pack<T>::none);
-    if (owns && sl.v0 + lane + 32 * i < sl.v1) u[i] = __ldg(sl.mid + sl.v0 + lane + 32 * i);
+    if (owns && sl.v0 + of + 32 * i < sl.v1) u[i] = __ldg(sl.mid + sl.v0 + of + 32 * i);
   }
+  if (SHORT) u[0] = part_of<T>(u[0], sub, lane & ((1 << sub) - 1));
   const float x_head = owns && lane < sl.head ? to_float<T>(sl.row[lane]) : -INFINITY;
   const float x_tail = owns && sl.tail + lane < sl.V ? to_float<T>(sl.row[sl.tail + lane]) : -INFINITY;
   // what the last part needs
@@ -543,7 +558,7 @@ step_kernel(const __grid_constant__ Params p) {
       } else if (one) {
         w = __ldg(sl.mid + best_at + lane);
       }
-      if (one) push_vector(w, best_at + lane);
+      if (one) push_vector(w, best_at + of);
     }
     #pragma unroll 1
     for (uint32_t todo = __ballot_sync(0xffffffffu, mine && in_others >= least); todo; todo &= todo - 1) {
@@ -873,7 +888,7 @@ sequences_kernel(const __grid_constant__ SequenceParams p) {
 }
 
 // What the current device says of a kernel, asked once.
-template <typename T>
+template <typename T, bool SHORT>
 struct Fit {
   int clusters[5];                       // resident clusters of 1, 2, 4, 8, 16 blocks
   static const Fit* get() {
@@ -882,7 +897,7 @@ struct Fit {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     if (const Fit* f = known[dev]) return f;
     Fit* f = new Fit;                    // kept for the life of the process (a second thread may find the same again)
-    if (!resident_clusters((const void*)step_kernel<T>, THREADS, 0, f->clusters)) { delete f; return nullptr; }
+    if (!resident_clusters((const void*)step_kernel<T, SHORT>, THREADS, 0, f->clusters)) { delete f; return nullptr; }
     known[dev] = f;
     return f;
   }
@@ -891,28 +906,34 @@ struct Fit {
 static int cluster_log2(int B, int K, int64_t bytes, const int (&clusters)[5]) {
   // The whole batch is resident; more blocks per sentence shorten its pass, 16 only where a slice would not fit a warp's
   // registers with 8 (a sentence of 4 x 32128 16-bit logits: 7.9 us with 8, 8.5 with 16; of 16 x 65537 float32: 26.7 and
-  // 21.6) and half of the blocks' places are enough.  A beam has two warps at least, for the number of groups that its
+  // 21.6) and one block per multiprocessor is enough.  A beam has two warps at least, for the number of groups that its
   // bound is taken from.
   int c = bytes > 8 * WARPS * 32 * 4 * 16 ? 4 : 3;
-  while (c > (K > 8 ? 1 : 0) && B > (c == 4 ? clusters[4] / 2 : clusters[c])) --c;
+  while (c > (K > 8 ? 1 : 0) && (B > clusters[c] || (c == 4 && B * 16ll > 148))) --c;
   return c;
+}
+
+template <typename T, bool SHORT>
+static int launch_blocks(const Params& p, cudaStream_t stream) {
+  if (!Fit<T, SHORT>::get()) return T5B_ERR_LAUNCH;                      // (which allows the launch such clusters)
+  const unsigned C = 1u << p.cluster_log2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.B * C); cfg.blockDim = dim3(THREADS); cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, step_kernel<T, SHORT>, p) == cudaSuccess ? T5B_OK : T5B_ERR_LAUNCH;
 }
 
 template <typename T>
 static int launch_step(Params p, cudaStream_t stream) {
-  const auto* fit = Fit<T>::get();
+  const auto* fit = Fit<T, false>::get();
   if (!fit) return T5B_ERR_LAUNCH;
   p.cluster_log2 = cluster_log2(p.B, p.K, (int64_t)p.K * p.V * sizeof(T), fit->clusters);
-  const int C = 1 << p.cluster_log2;
-  p.S = C * WARPS / p.K;
+  p.S = (WARPS << p.cluster_log2) / p.K;
   p.unit_magic = (65536u + p.S - 1) / p.S; p.slice_magic = (uint32_t)(((1ull << 32) + p.S - 1) / p.S);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.B * C)); cfg.blockDim = dim3(THREADS); cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)C; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr; cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, step_kernel<T>, p) == cudaSuccess ? T5B_OK : T5B_ERR_LAUNCH;
+  return p.V / Pack<T>::N / p.S + 1 <= 16 ? launch_blocks<T, true>(p, stream) : launch_blocks<T, false>(p, stream);
 }
 
 }  // namespace beam
