@@ -1,0 +1,33 @@
+"""CPU checks of the generation kernels' sources and C entry points: what must not be found out on a device."""
+import os
+import re
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _kernel(source, name):
+    """The text of a __global__ function without comments."""
+    text = open(os.path.join(ROOT, "turbot5_b200", "csrc", source)).read()
+    text = re.sub(r"//[^\n]*", "", text)
+    at = text.index("{", re.search(r"\b%s\(const __grid_constant__" % name, text).start())
+    depth = 0
+    for i in range(at, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if depth == 0:
+            return text[at:i + 1]
+
+
+def _depth(text, at):
+    return text[:at].count("{") - text[:at].count("}")
+
+
+def test_step_writes_to_the_first_block_only_behind_a_barrier():
+    """A block may write another's shared memory once that block has started, and words that the owner clears itself only
+    behind the clearing: every thread arrives after the clearing and waits before the first access through `lead`."""
+    body = _kernel("beam_search.cu", "step_kernel")
+    cleared, arrive, wait = body.index("sm.counts[tid] = 0"), body.index("cluster_arrive()"), body.index("cluster_wait()")
+    first = min(m.start() for m in re.finditer(r"lead->|map_shared_rank\(&sm, (?!0\))", body))
+    assert cleared < arrive < wait < first
+    assert max(body.index(w) for w in ("sm.found_here = 0", "sm.overflow = 0", "sm.kept = 0", "sm.threshold = 0")) < arrive
+    # by every thread of every block that stays: on the function's own level, with no way out between the two
+    assert _depth(body, arrive) == _depth(body, wait) == 1 and "return" not in body[arrive:wait]

@@ -801,3 +801,15 @@ def test_step_of_small_vocabularies(B, K, V, dtype):
             rows = flat[offset:].view(B * K, V + offset)[:, :V]
         s = _search(B, K, 42, 3)
         _check_step(_run_step(rows if offset else rows.cuda(), s), x, s)
+
+
+def test_step_of_many_short_launches_gives_the_same_bits():
+    """Launches one behind the other whose pass is next to nothing, so that a cluster's blocks start and write at almost the
+    same time."""
+    logits, s = _logits(60, 4, 40, torch.bfloat16, 13), _search(60, 4, 12, 4)
+    want = _run_step(logits.cuda(), s)
+    _check_step(want, logits, s)
+    import turbot5_b200 as t5b
+    dev, pos, x = [s[n].cuda() for n in ("scores", "pool", "steps", "beams", "done")], torch.tensor([s["pos"]], device="cuda"), logits.cuda()
+    every = [t5b.beam_search_step(x, *dev, pos) for _ in range(400)]
+    assert all(torch.equal(a, b) for got in every for a, b in zip(got, want))

@@ -9,7 +9,8 @@
 //
 // One cluster of blocks per sentence reads every logit once; a warp owns a slice of one beam's row (a "unit").
 // What a kernel of this size costs is not the bytes but the steps that wait for one another (a cluster barrier is some 900
-// cycles, as much as the exponentials of a block's 32 KB), so there is one exchange:
+// cycles, as much as the exponentials of a block's 32 KB), so there is one exchange (and before the first word of it a
+// barrier that says that every block has started: arrived at before the pass over the logits, waited for behind it):
 //
 //   * In a block, the warps of one row form a segment.  The n-th largest of the maxima of groups of its lanes is a bound
 //     that n of its elements reach, so only lanes whose own maximum reaches it look at their elements again: for n = 8
@@ -202,6 +203,10 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+
+// The two halves of a barrier of the cluster: what a block wrote before the first is seen behind the second by all.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // Sum of exponentials of a slice that holds NaN (left out) or +inf (counted): rare, and kept out of the way.
 template <typename T>
@@ -470,6 +475,9 @@ step_kernel(const __grid_constant__ Params p) {
   int best_at = 0;
   if (tid == 0) { sm.found_here = 0; sm.overflow = 0; sm.kept = 0; sm.threshold = 0; }
   if (tid < MAX_CLUSTER) sm.counts[tid] = 0;
+  cluster_arrive();
+  float wm = -INFINITY;
+  double total = 0.0;
   if (active) {
     m = fmaxf(fmaxf(x_head, x_tail), -INFINITY);         // (NaN only: -inf)
     const float edge = m > -INFINITY ? m : 0.f;
@@ -509,15 +517,16 @@ step_kernel(const __grid_constant__ Params p) {
           s += (part[0] + part[1]) + (part[2] + part[3]);
         }
     }
-    const float wm = warp_max(m);
-    double total;
+    wm = warp_max(m);
     if (__any_sync(0xffffffffu, !(s == s) || m == INFINITY)) {      // NaN or +inf among the logits
       total = careful_sum<T>(sl, wm, lane);
     } else {
       total = warp_sum(wm > -INFINITY ? (double)(s * fast_exp2((m - wm) * kLog2e)) : 0.0);
     }
-    if (lane == 0) { lead->umax[unit] = wm; lead->usum[unit] = total; }
   }
+  // every block has started and has cleared its counts: from here on the first one's memory may be written
+  cluster_wait();
+  if (active && lane == 0) { lead->umax[unit] = wm; lead->usum[unit] = total; }
 
   // ---- the candidates of this block's segments
   const int first = active ? max(k * S - rank * WARPS, 0) : warp;                    // the segment's warps
