@@ -31,3 +31,12 @@ def test_step_writes_to_the_first_block_only_behind_a_barrier():
     assert max(body.index(w) for w in ("sm.found_here = 0", "sm.overflow = 0", "sm.kept = 0", "sm.threshold = 0")) < arrive
     # by every thread of every block that stays: on the function's own level, with no way out between the two
     assert _depth(body, arrive) == _depth(body, wait) == 1 and "return" not in body[arrive:wait]
+
+
+def test_warps_of_the_step_leave_a_loop_together():
+    """Other warps add to the number of candidates while a warp reads it: were it read by every lane for itself, some could
+    leave the loop and others wait for them at its end.  Between the lanes' reads and the way out stands a broadcast."""
+    body = _kernel("beam_search.cu", "step_kernel")
+    pushes = body[body.index("cluster_wait()"):body.index("cluster.sync()")]
+    ways_out = [line for line in pushes.splitlines() if "break" in line]
+    assert len(ways_out) == 1 and re.search(r"if \(__shfl_sync\(0xffffffffu, [^;]*found_here, 0\) > share\) break;", ways_out[0])

@@ -571,7 +571,8 @@ step_kernel(const __grid_constant__ Params p) {
     }
     #pragma unroll 1
     for (uint32_t todo = __ballot_sync(0xffffffffu, mine && in_others >= least); todo; todo &= todo - 1) {
-      if (sm.found_here > share) break;                  // more than can be used: the lists will do it
+      // more than can be used: the lists will do it (other warps add to the number: what one lane has read holds)
+      if (__shfl_sync(0xffffffffu, *(volatile int*)&sm.found_here, 0) > share) break;
       const int who = __ffs(todo) - 1;                   // several: its vectors again, by the whole warp
       #pragma unroll 1
       for (int v = sl.v0 + who + 32 * lane; v < sl.v1; v += 32 * 32) push_vector(__ldg(sl.mid + v), v);
