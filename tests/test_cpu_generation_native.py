@@ -21,16 +21,22 @@ def _depth(text, at):
     return text[:at].count("{") - text[:at].count("}")
 
 
-def test_step_writes_to_the_first_block_only_behind_a_barrier():
-    """A block may write another's shared memory once that block has started, and words that the owner clears itself only
-    behind the clearing: every thread arrives after the clearing and waits before the first access through `lead`."""
+def test_step_writes_to_the_first_block_only_once_it_has_started():
+    """A block may write another's shared memory once that block has started: every thread arrives at the beginning and
+    waits before the first access through `lead`.  What is written there the first block does not set itself: nothing would
+    order the two."""
     body = _kernel("beam_search.cu", "step_kernel")
-    cleared, arrive, wait = body.index("sm.counts[tid] = 0"), body.index("cluster_arrive()"), body.index("cluster_wait()")
+    arrive, wait, exchange = body.index("cluster_arrive()"), body.index("cluster_wait()"), body.index("cluster.sync()")
     first = min(m.start() for m in re.finditer(r"lead->|map_shared_rank\(&sm, (?!0\))", body))
-    assert cleared < arrive < wait < first
-    assert max(body.index(w) for w in ("sm.found_here = 0", "sm.overflow = 0", "sm.kept = 0", "sm.threshold = 0")) < arrive
+    assert arrive < wait < first < exchange
     # by every thread of every block that stays: on the function's own level, with no way out between the two
     assert _depth(body, arrive) == _depth(body, wait) == 1 and "return" not in body[arrive:wait]
+    written = set(re.findall(r"lead->(\w+)", body))
+    assert written == {"umax", "usum", "reached", "found", "counts"}
+    own = set(re.findall(r"\bsm\.(\w+)", body[:exchange]))
+    assert not written & own, written & own
+    # counts: of the blocks that there are only
+    assert re.search(r"= r < C \? sm\.counts\[r\] : 0;", body)
 
 
 def test_warps_of_the_step_leave_a_loop_together():

@@ -204,8 +204,10 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// The two halves of a barrier of the cluster: what a block wrote before the first is seen behind the second by all.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+// The two halves of a barrier of the cluster that says that every block has started.  Nothing that is written before it is
+// read by another block, so it orders no memory (with a release 0.3 to 0.8 us of the step went to it: the fence waits for
+// the logits' first reads).
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // Sum of exponentials of a slice that holds NaN (left out) or +inf (counted): rare, and kept out of the way.
@@ -474,7 +476,6 @@ step_kernel(const __grid_constant__ Params p) {
   float m = -INFINITY, in_best = -INFINITY, in_others = -INFINITY;
   int best_at = 0;
   if (tid == 0) { sm.found_here = 0; sm.overflow = 0; sm.kept = 0; sm.threshold = 0; }
-  if (tid < MAX_CLUSTER) sm.counts[tid] = 0;
   cluster_arrive();
   float wm = -INFINITY;
   double total = 0.0;
@@ -524,7 +525,7 @@ step_kernel(const __grid_constant__ Params p) {
       total = warp_sum(wm > -INFINITY ? (double)(s * fast_exp2((m - wm) * kLog2e)) : 0.0);
     }
   }
-  // every block has started and has cleared its counts: from here on the first one's memory may be written
+  // every block has started: from here on the first one's memory may be written, where it writes nothing itself
   cluster_wait();
   if (active && lane == 0) { lead->umax[unit] = wm; lead->usum[unit] = total; }
 
@@ -616,7 +617,7 @@ step_kernel(const __grid_constant__ Params p) {
     bool fits = true;
     #pragma unroll
     for (int r = 0; r < MAX_CLUSTER; ++r) {
-      const int c = sm.counts[r];
+      const int c = r < C ? sm.counts[r] : 0;            // (each block has written its own)
       fits = fits && c <= share;
       before += r < (warp & (C - 1)) ? c : 0;
       total += c;
