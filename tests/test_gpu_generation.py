@@ -813,3 +813,62 @@ def test_step_of_many_short_launches_gives_the_same_bits():
     dev, pos, x = [s[n].cuda() for n in ("scores", "pool", "steps", "beams", "done")], torch.tensor([s["pos"]], device="cuda"), logits.cuda()
     every = [t5b.beam_search_step(x, *dev, pos) for _ in range(400)]
     assert all(torch.equal(a, b) for got in every for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,M,N", [(64, 1, 2000), (64, 4, 16384), (64, 7, 2000), (16, 2, 5000), (32, 8, 3000), (128, 1, 16384), (128, 5, 2000),
+                                   (64, 1, 100000), (128, 3, 40)])
+@pytest.mark.parametrize("nats", [10.12, 17.5, 22.0])
+def test_attention_faint_tail_behind_a_leading_key(nats, D, M, N, dtype):
+    """One key that takes nearly all of the weight, with values of 0: the result is that of the others, e^-nats each."""
+    import turbot5_b200 as t5b
+    cap = -(-N // 64) * 64
+    g = torch.Generator().manual_seed(N)
+    for lead in {0, N // 2, N - 1}:
+        k, v = torch.zeros((1, 1, cap, D)), torch.rand((1, 1, cap, D), generator=g).add(1).mul(200).to(FP8).float()
+        k[0, 0, lead, 0] = 1.0
+        v[0, 0, lead] = 0
+        # rows of their own: 16 / 16, 15 / 16, ... of the leading key's score; the first row's result is about 1
+        q = torch.zeros((1, 1, M, D))
+        q[0, 0, :, 0] = 1 - torch.arange(M) / 16
+        v_scale = 2.0 ** round(math.log2(math.exp(nats) / N / 300))
+        ks, vs = torch.ones((1, 1, cap // 64)), torch.full((1, 1, cap // 64), v_scale)
+        got = t5b.flash_decoding_quantized_with_fusing_bias(q.to(dtype).cuda(), k.to(FP8).cuda(), ks.cuda(), v.to(FP8).cuda(), vs.cuda(), None,
+                                                            sm_scale=nats, kv_len=N)[0, 0].double().cpu()
+        tail = v[0, 0, :N].double().sum(0) * v_scale
+        for m in range(M):
+            faint = math.exp(-nats * (1 - m / 16))
+            total = 1 + faint * (N - 1)
+            want = tail * faint / total
+            # per weight: its two halves 2^-22, two exponentials of 2^-22 (its own, its item's), their arguments (up to
+            # 1.5 nats + 14 each, rounded twice); sums of an item, of a warp's items and of the warps in float32; keys that
+            # share the leading key's item: half of 2^-38 of its weight (rounding of hi and of lo, at 2^14: 2^-25 each)
+            steps = N / (32 * 8) + 2 + 64 + 64
+            rel = 3 * 2.0 ** -22 + 4 * (1.5 * nats + 14) * 2.0 ** -24 + 2 * steps * 2.0 ** -23
+            tol = want * (torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -8) + rel) + 63 * 2.0 ** -38 * 400 * v_scale / total
+            off = (got[m] - want).abs()
+            assert (off <= tol).all(), (lead, m, (off / want).max(), (tol / want).min())
+
+
+@pytest.mark.parametrize("D,M", [(64, 1), (64, 6), (128, 2)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_equal_scores_of_any_size(D, M, sign):
+    """Equal scores give the mean of the values, however large they are (their last place may be wider than the 14 that
+    weights are kept above 1); a second group of keys far below takes no part."""
+    import turbot5_b200 as t5b
+    N = 150
+    (k, _), (v, vs) = _cache(1, 2, 192, D, 3), _cache(1, 2, 192, D, 4)
+    k = torch.zeros_like(k.float())
+    k[..., 0] = sign
+    k[:, :, 64:100, 0] = -2
+    q = torch.zeros((1, 2, M, D))
+    q[..., 0] = 1
+    kept = [n for n in range(N) if not 64 <= n < 100]
+    want = (v.double() * vs.double().repeat_interleave(64, -1)[..., None])[:, :, kept]
+    want, size = want.mean(2, keepdim=True), want.abs().mean(2, keepdim=True)
+    for power in (9, 18, 19, 20, 21, 24, 25, 26, 27, 30, 60, 100):
+        got = t5b.flash_decoding_quantized_with_fusing_bias(q.half().cuda(), k.to(FP8).cuda(), torch.ones((1, 2, 3), device="cuda"), v.cuda(), vs.cuda(),
+                                                            None, sm_scale=2.0 ** power, kv_len=N).double().cpu()
+        # float32 sums of 150 numbers (each half of a weight exact), a quotient, the result's rounding
+        tol = want.abs() * 2.0 ** -11 * (1 + 2.0 ** -8) + size * 200 * 2.0 ** -23 + 2.0 ** -25
+        assert ((got - want).abs() <= tol).all(), power

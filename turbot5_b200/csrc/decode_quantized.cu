@@ -16,12 +16,16 @@
 //   * P^T comes out of S^T's registers by one 8x8 transpose of 16-bit pairs.
 //   * fp16 products of e4m3 numbers are exact in float32; q is scaled to 1 by a power of two.  P is carried as hi + lo:
 //     with up to four rows, row r has columns 2r and 2r + 1 of the product, one for each half (a lane then makes the
-//     weights of one row only); with up to eight rows the product is issued twice.  P keeps 22 bits, so the result is
-//     as exact as float32 weights would make it.
+//     weights of one row only); with up to eight rows the product is issued twice.  An item's weights are made relative to
+//     its own largest one, which is 2^14: hi + lo then hold 22 bits of every weight down to 2^-17 of that, and 2^-39 of it
+//     below.  (Relative to a running maximum of 1 the weights of a long faint tail behind one leading key fell among fp16's
+//     subnormal numbers: up to 2e-3 of the result at 2^-15, all of it below 2^-25.)
 //
 // A warp works on items of 32 or 64 keys of one block of 64 (so an item has one scale), with its own running maximum and
 // sum and its own ring of stages in shared memory that asynchronous copies fill ahead (registers alone held too little in
-// flight: 206 us instead of 167 for 1.07 GB, 98 % of the measured copy rate).  Warps merge in shared memory, the blocks
+// flight: 206 us for 1.07 GB, 166 with the ring, the floor at the measured copy rate 164).  That is at 1965 MHz, in bursts
+// of some milliseconds.  A second of it draws the 1000 W that the GPU may take, the clock falls to 1450 MHz and issue slots
+// decide: 188 us, 193 as calls one behind the other.  Warps merge in shared memory, the blocks
 // of a (batch, head) that share a long cache form a cluster and merge through distributed shared memory: no workspace,
 // no counters, no second launch.  The bias is looked up for items within the largest distance of a query only, from a
 // table of the item's distances that the warp makes for itself.
@@ -40,6 +44,7 @@ namespace t5b {
 namespace decq {
 
 constexpr int BLOCK = T5B_CACHE_BLOCK;
+constexpr float LOWEST = -3.402823466e38f;   // where a running maximum starts: finite, so that differences from it are numbers
 // 16-key tiles of an item, and how its stages lie in shared memory: keys, values, two scales
 template <int D> struct Ring {
   static constexpr int SUB = D == 128 ? 2 : D == 64 ? 2 : 4;
@@ -253,7 +258,7 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
 
   float m_run[COLS], l_run[COLS];
   #pragma unroll
-  for (int i = 0; i < COLS; ++i) { m_run[i] = -INFINITY; l_run[i] = 0.f; }
+  for (int i = 0; i < COLS; ++i) { m_run[i] = LOWEST; l_run[i] = 0.f; }
   float acc[TILES][KSTEPS][4];
   #pragma unroll
   for (int t = 0; t < TILES; ++t)
@@ -329,19 +334,22 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
         if (!whole && (n0 + key >= n_end || (p.causal && n0 + key > col_pos[i]))) s[t][e] = -INFINITY;
         mx[i] = fmaxf(mx[i], s[t][e]);
       }
-    // ---- running maximum, weights
-    float alpha[COLS], ref[COLS];
+    // ---- running maximum, weights: those of an item relative to its own largest one, 2^14, and `beta` from there to the
+    // running maximum (scores beyond 2^20, whose steps are too wide for the 14, relative to 1)
+    float alpha[COLS], beta[COLS], ref[COLS];
     #pragma unroll
     for (int i = 0; i < COLS; ++i) {
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 4));
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 8));
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 16));
       const float m_new = fmaxf(m_run[i], mx[i]);
-      ref[i] = m_new == -INFINITY ? 0.f : m_new;
-      alpha[i] = fast_exp2(m_run[i] - ref[i]);
+      ref[i] = fmaxf(mx[i], LOWEST);
+      if (fabsf(ref[i]) < 1048576.f) ref[i] -= 14.f;
+      alpha[i] = fast_exp2(m_run[i] - m_new);
+      beta[i] = fast_exp2(ref[i] - m_new);
       m_run[i] = m_new;
-      l_run[i] *= alpha[i];
     }
+    float sum[COLS];
     float part[TILES][KSTEPS][4];
     #pragma unroll
     for (int t = 0; t < TILES; ++t)
@@ -355,7 +363,7 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
       #pragma unroll
       for (int e = 0; e < 2 * COLS; ++e) {
         w[e] = fast_exp2(s[t][e] - ref[e % COLS]);
-        l_run[e % COLS] += w[e];
+        sum[e % COLS] = t == 0 && e < COLS ? w[e] : sum[e % COLS] + w[e];
         hi[e] = __uint_as_float(__float_as_uint(w[e]) & 0xffffe000u);
         lo[e] = w[e] - hi[e];
       }
@@ -384,11 +392,16 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
       }
     }
     #pragma unroll
+    for (int i = 0; i < COLS; ++i) {
+      l_run[i] = fmaf(sum[i], beta[i], l_run[i] * alpha[i]);
+      beta[i] *= v_scale;
+    }
+    #pragma unroll
     for (int t = 0; t < TILES; ++t)
       #pragma unroll
       for (int i = 0; i < KSTEPS; ++i)
         #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][i][e] = fmaf(part[t][i][e], v_scale, acc[t][i][e] * alpha[TILES == 1 ? 0 : e & 1]);
+        for (int e = 0; e < 4; ++e) acc[t][i][e] = fmaf(part[t][i][e], beta[TILES == 1 ? 0 : e & 1], acc[t][i][e] * alpha[TILES == 1 ? 0 : e & 1]);
   }
   copy_wait<0>();
   __syncwarp();                          // the ring is free for the warp's result
