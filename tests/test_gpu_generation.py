@@ -872,3 +872,32 @@ def test_attention_equal_scores_of_any_size(D, M, sign):
         # float32 sums of 150 numbers (each half of a weight exact), a quotient, the result's rounding
         tol = want.abs() * 2.0 ** -11 * (1 + 2.0 ** -8) + size * 200 * 2.0 ** -23 + 2.0 ** -25
         assert ((got - want).abs() <= tol).all(), power
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,M", [(16, 1), (64, 4), (64, 8), (128, 1)])
+def test_attention_small_elements_of_a_query_beside_a_large_one(D, M, dtype):
+    """The keys are 0 where the query is large: its small elements alone make the scores."""
+    B, H, n = 2, 2, 130
+    g = torch.Generator().manual_seed(D + M)
+    for power in (-12, -20, -24):                      # (held exactly down to 2^-31 of the row's largest element)
+        q = torch.randn((B, H, M, D), generator=g) * 2.0 ** power
+        q[..., 3] = 1.0
+        (k, ks), kv_v = _cache(B, H, 192, D, 3), _cache(B, H, 192, D, 4)
+        kf = k.float()
+        kf[..., 3] = 0
+        # scores of a few units; float16 holds no elements below 2^-24: the large one is then 2^14
+        lift = 2.0 ** 14 if dtype == torch.float16 else 1.0
+        _check_attention((q * lift).to(dtype), ((kf.to(FP8), torch.full_like(ks, 2.0 ** -6)), kv_v), None, [n, 60], False,
+                         2.0 ** -power / lift * D ** -0.5)
+
+
+@pytest.mark.parametrize("power", [-133, -126, -112, 100, 124, 126])
+def test_attention_queries_of_any_size(power):
+    """From subnormal numbers to the largest ones, with scales and a factor that make ordinary scores of them."""
+    B, H, M, D, n = 1, 2, 3, 64, 100
+    g = torch.Generator().manual_seed(5)
+    q = (torch.randn((B, H, M, D), generator=g).clamp(-1.9, 1.9).double() * 2.0 ** power).to(torch.bfloat16)
+    (k, ks), kv_v = _cache(B, H, 128, D, 3), _cache(B, H, 128, D, 4)
+    half = 2.0 ** (-power // 2)
+    _check_attention(q, ((k, torch.full_like(ks, 2.0 ** -8 * half)), kv_v), None, [n], False, 2.0 ** -power / half)

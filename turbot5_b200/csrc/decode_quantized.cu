@@ -14,7 +14,8 @@
 //   * O^T = V^T P^T: the head dim is the rows.  A byte permute joins two keys' bytes to pairs along the key dim.  Which
 //     key is which row of a 16-key tile is free as well: the order is such that reading values has no bank conflicts.
 //   * P^T comes out of S^T's registers by one 8x8 transpose of 16-bit pairs.
-//   * fp16 products of e4m3 numbers are exact in float32; q is scaled to 1 by a power of two.  P is carried as hi + lo:
+//   * fp16 products of e4m3 numbers are exact in float32; a row of q is scaled by a power of two to 2^15 at most, which holds
+//     bf16 exactly down to 2^-31 of the row's largest element (fp16 2^-28), and to 2^-39 of it below.  P is carried as hi + lo:
 //     with up to four rows, row r has columns 2r and 2r + 1 of the product, one for each half (a lane then makes the
 //     weights of one row only); with up to eight rows the product is issued twice.  An item's weights are made relative to
 //     its own largest one, which is 2^14: hi + lo then hold 22 bits of every weight down to 2^-17 of that, and 2^-39 of it
@@ -216,7 +217,7 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
   #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) request(it + i * step, i);
 
-  // ---- queries, scaled to at most 1
+  // ---- queries, scaled to fp16's upper end
   uint32_t qf[KSTEPS][2];
   float col_scale[COLS];                 // of this lane's rows: c (TILES 1) or 2c and 2c + 1
   int col_pos[COLS];
@@ -233,9 +234,8 @@ decode_quantized_kernel(const __grid_constant__ Params p, const __grid_constant_
     }
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    // a power of two at or below the largest element (1 where that is 0, tiny or not finite)
-    const uint32_t eb = __float_as_uint(most) & 0x7f800000u;
-    const float unit = eb >= 0x01000000u && eb <= 0x7e000000u ? __uint_as_float(eb) : 1.f;
+    // a power of two: the largest element becomes 2^14 .. 2^15 (or less, of rows below 2^-111)
+    const float unit = __uint_as_float(max(__float_as_uint(most) & 0x7f800000u, 0x08000000u) - (14u << 23));
     const float inv = 1.f / unit;
     #pragma unroll
     for (int j = 0; j < KSTEPS; ++j) {
