@@ -416,8 +416,8 @@ T5B_API int t5b_scatter_rows(const void* packed, int64_t packed_row_stride_bytes
  * done: the pool is full and early_stopping, or no running score / (pos + 1)^length_penalty is above the pool's worst;
  * or every running score is -inf.  A sentence that is done on entry keeps scores and pool, its tokens are pad_token_id,
  * its parents itself.
- * NaN logits count as -inf; a row with +inf gives those tokens the whole probability.  Scores are float32, computed and
- * compared in float64.
+ * NaN logits count as -inf; a row with +inf gives those tokens the whole probability.  Scores are float32, compared in
+ * float64 before they are rounded; a row's log-sum comes from float32 exponentials and is good to about 1.4e-7.
  *   logits (B * num_beams, vocab), row stride in elements, 2 <= vocab <= 2^27; pos: int64 device word, the step's number
  *   from 0; finished_steps / finished_beams: the step and the parent beam of each finished sentence's end.
  *   *_out may be the inputs.  history_*: optional int32 (history_steps, B, num_beams), row pos is written. */

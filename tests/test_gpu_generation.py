@@ -901,3 +901,29 @@ def test_attention_queries_of_any_size(power):
     (k, ks), kv_v = _cache(B, H, 128, D, 3), _cache(B, H, 128, D, 4)
     half = 2.0 ** (-power // 2)
     _check_attention(q, ((k, torch.full_like(ks, 2.0 ** -8 * half)), kv_v), None, [n], False, 2.0 ** -power / half)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,K,V,std", [(100, 16, 128256, 6.0), (16, 4, 32128, 2.5), (40, 16, 32128, 1.0)])
+def test_step_log_sums(B, K, V, std, dtype):
+    """Running scores that cancel the log-probability of each row's best token: what is left is the error of the log-sum, not
+    hidden by the rounding of the result."""
+    import turbot5_b200 as t5b
+    g = torch.Generator(device="cuda").manual_seed(V)
+    logits = (torch.randn((B * K, V), generator=g, device="cuda") * std).to(dtype)
+    lse = torch.cat([torch.logsumexp(rows.double(), -1) for rows in logits.split(64)])
+    scores = (lse - logits.max(-1)[0].double()).float()
+    none = torch.zeros((B, K), dtype=torch.int32, device="cuda")
+    tokens, parents, out, *_ = t5b.beam_search_step(logits, scores.view(B, K), torch.full((B, K), NONE, device="cuda"), none, none,
+                                                    torch.zeros(B, dtype=torch.bool, device="cuda"), torch.zeros(1, dtype=torch.long, device="cuda"),
+                                                    eos_token_id=None)
+    rows = (torch.arange(B, device="cuda")[:, None] * K + parents.long()).flatten()
+    want = scores[rows].double() + (logits[rows, tokens.flatten()].double() - lse[rows])
+    off = (out.flatten().double() - want)[want.abs() < 1e-3]           # (float32 of 1e-3: 2^-34)
+    assert off.numel() >= B * K // 2
+    # at most: four exponentials in a row (a term's, those to its lane's, its warp's and the row's maximum) of 2^-22, their
+    # arguments (up to 40 in base 2, three roundings), 12 float32 additions
+    assert off.abs().max() <= 4 * 2.0 ** -22 + 3 * 40 * 2.0 ** -24 * math.log(2) + 12 * 2.0 ** -24
+    # on average the roundings cancel.  What remains: an exponential is 5.1e-8 too small (three of them), and log2(e) in
+    # float32 1.4e-8 of the distance from the maximum (3 on the weighted average)
+    assert off.mean().abs() <= 3 * 5.1e-8 + 3 * 1.4e-8

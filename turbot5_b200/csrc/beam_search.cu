@@ -21,14 +21,17 @@
 //   * Where that fails - fewer finite candidates than n, or hundreds of equal ones - every warp makes the sorted list of its
 //     slice's n best instead and the first block merges the lists.
 //
-// Sums of exponentials are float32 within a lane (a few dozen terms) and float64 from there on, as are the scores: two
-// candidates of different beams are told apart to about 1e-8.
+// Exponentials are float32 (off by 2^-22 at most, 5e-8 too small on average, and by the rounding of their arguments), 32 of a
+// lane are summed in float32, everything from there on and the scores in float64.  Log-sums came out within 1.4e-7 of the
+// exact ones (rows of 1000 to 250112 logits, of standard deviation 0.3 to 6, and peaked ones): candidates of different beams
+// are told apart to that, those of one beam exactly.  (With a lane's whole sum in float32 1.6e-6 where it had 2000 terms.)
 //
-// Measured on B200 (device time, launches in a graph): 6.8 us for one sentence of 4 beams x 32128 bf16 logits, 11.3 us for
-// 64 of them (16.4 MB), 20.9 us for 8 sentences of 16 beams x 65537 float32 logits (33.6 MB; the pass itself 5.8 us, at
+// Measured on B200 (device time, launches in a graph): 7.1 us for one sentence of 4 beams x 32128 bf16 logits, 11.6 us for
+// 64 of them (16.4 MB), 21.1 us for 8 sentences of 16 beams x 65537 float32 logits (33.6 MB; the pass itself 5.8 us, at
 // the copy rate).  Of the first, about 1400 cycles are the first reads, 2100 the exponentials (one unit of 16 a clock),
-// 1000 the barrier, 8000 the short steps around it.  A second exchange with a bound over the whole sentence, float64
-// second looks and unrolled one-shot code (126 KB) cost 9.0, 12.0 and 9.2 us.
+// 1000 the barrier, 8000 the short steps around it; that every block has started costs 0.1 to 0.2 us of them, the sums in
+// float64 0.07.  A second exchange with a bound over the whole sentence, float64 second looks and unrolled one-shot code
+// (126 KB) cost 9.0, 12.0 and 9.2 us.
 //
 // The reference has no beam search of its own (its heads inherit it: src/turbot5/heads/t5_heads.py:100-130).
 #include "t5b_common.cuh"
@@ -482,7 +485,7 @@ step_kernel(const __grid_constant__ Params p) {
   if (active) {
     m = fmaxf(fmaxf(x_head, x_tail), -INFINITY);         // (NaN only: -inf)
     const float edge = m > -INFINITY ? m : 0.f;
-    float s = fast_exp2((x_head - edge) * kLog2e) + fast_exp2((x_tail - edge) * kLog2e);
+    double s = fast_exp2((x_head - edge) * kLog2e) + fast_exp2((x_tail - edge) * kLog2e);
     #pragma unroll 1
     for (int v = sl.v0; v < sl.v1; v += 32 * U) {
       float m_new = m;
@@ -499,8 +502,9 @@ step_kernel(const __grid_constant__ Params p) {
           m_new = fmaxf(m_new, most);
         }
       const float ref = m_new > -INFINITY ? m_new : 0.f;
-      s *= fast_exp2((m - ref) * kLog2e);
+      const double moved = fast_exp2((m - ref) * kLog2e);
       m = m_new;
+      float batch = 0.f;
       const bool more = v + 32 * U < sl.v1;
       #pragma unroll
       for (int i = 0; i < U; ++i)
@@ -515,14 +519,15 @@ step_kernel(const __grid_constant__ Params p) {
           float part[4] = {0.f, 0.f, 0.f, 0.f};
           #pragma unroll
           for (int e = 0; e < N; ++e) part[e & 3] += fast_exp2((x[e] - ref) * kLog2e);
-          s += (part[0] + part[1]) + (part[2] + part[3]);
+          batch += (part[0] + part[1]) + (part[2] + part[3]);
         }
+      s = s * moved + batch;
     }
     wm = warp_max(m);
     if (__any_sync(0xffffffffu, !(s == s) || m == INFINITY)) {      // NaN or +inf among the logits
       total = careful_sum<T>(sl, wm, lane);
     } else {
-      total = warp_sum(wm > -INFINITY ? (double)(s * fast_exp2((m - wm) * kLog2e)) : 0.0);
+      total = warp_sum(wm > -INFINITY ? s * (double)fast_exp2((m - wm) * kLog2e) : 0.0);
     }
   }
   // every block has started: from here on the first one's memory may be written, where it writes nothing itself

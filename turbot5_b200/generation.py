@@ -21,8 +21,8 @@ def beam_search_step(logits, scores, finished_scores, finished_steps, finished_b
 
     `logits` (batch * num_beams, vocab) in float32, float16 or bfloat16 are those of the running beams, whose summed
     log-probabilities are `scores` (batch, num_beams) float32 (start with 0 for one beam of a sentence and -inf for the
-    others).  The candidates are the 2 * num_beams best continuations by score + log_softmax(logits), computed and compared
-    in float64; among equal scores the lowest beam, within a beam the largest logit, then the lowest token.
+    others).  The candidates are the 2 * num_beams best continuations by score + log_softmax(logits), compared in float64 (a
+    row's log-sum comes from float32 exponentials and is good to about 1.4e-7); among equal scores the lowest beam, within a beam the largest logit, then the lowest token.
     A candidate that is `eos_token_id` (None: there is no such token) and among the num_beams best joins the pool of
     finished sentences with score / (pos + 1) ** length_penalty; `finished_scores` (float32, best first, -inf where
     empty), `finished_steps` and `finished_beams` (int32: step and parent beam of the end token) hold the num_beams
