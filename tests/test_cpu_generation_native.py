@@ -1,6 +1,8 @@
 """CPU checks of the generation kernels' sources and C entry points: what must not be found out on a device."""
 import os
 import re
+import subprocess
+import sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -46,3 +48,18 @@ def test_warps_of_the_step_leave_a_loop_together():
     pushes = body[body.index("cluster_wait()"):body.index("cluster.sync()")]
     ways_out = [line for line in pushes.splitlines() if "break" in line]
     assert len(ways_out) == 1 and re.search(r"if \(__shfl_sync\(0xffffffffu, [^;]*found_here, 0\) > share\) break;", ways_out[0])
+
+
+def _status(call):
+    """The status of a C entry point, asked in a process of its own: what ends it ends no test."""
+    code = "import ctypes\nfrom tests.test_cpu_host_side import _c_struct\nfrom turbot5_b200 import _native as nat\nL = nat.lib()\n" \
+           "ptr = lambda a: ctypes.cast(ctypes.byref(a), ctypes.c_void_p)\nprint('status', " + call + ")"
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, (r.returncode, r.stderr[-500:])
+    return int(r.stdout.split()[-1])
+
+
+def test_scales_are_reordered_with_their_caches_only():
+    """Without caches there is nothing to share blocks by."""
+    assert _status("L.t5b_beam_cache_reorder(ptr(_c_struct('t5b_cache_reorder_args')(n_caches=0, n_scales=1, outer=2, B=1, num_beams=4, H=2, "
+                   "capacity=64, token_bytes=64, parents=16, scales=(ctypes.c_void_p * 64)(16))), None)") == 5

@@ -383,7 +383,7 @@ extern "C" int t5b_beam_cache_reorder(const t5b_cache_reorder_args* a, void* str
       a->n_scales < 0 || a->token_bytes < 1 || a->n_caches > T5B_REORDER_MAX_TENSORS || a->n_scales > T5B_REORDER_MAX_TENSORS ||
       a->B > 65535 || (int64_t)(a->n_caches + a->n_scales) * a->outer > 65535) return T5B_ERR_SHAPE;
   if (a->B == 0 || a->H == 0 || a->capacity == 0 || a->outer == 0 || a->n_caches + a->n_scales == 0) return T5B_OK;
-  if (!a->parents) return T5B_ERR_ARG;
+  if (!a->parents || a->n_caches == 0) return T5B_ERR_ARG;         // scales go with their caches: heads set the grid
   kvcache::ReorderParams p;
   kvcache::ReorderGroup& c = p.g[0];
   kvcache::ReorderGroup& s = p.g[1];
