@@ -63,3 +63,11 @@ def test_scales_are_reordered_with_their_caches_only():
     """Without caches there is nothing to share blocks by."""
     assert _status("L.t5b_beam_cache_reorder(ptr(_c_struct('t5b_cache_reorder_args')(n_caches=0, n_scales=1, outer=2, B=1, num_beams=4, H=2, "
                    "capacity=64, token_bytes=64, parents=16, scales=(ctypes.c_void_p * 64)(16))), None)") == 5
+
+
+def test_numbers_of_tokens_near_the_largest_number_are_refused():
+    """The number of blocks that they fill is not computed beyond 2^31."""
+    full = ", ".join("%s=16" % n for n in ("k", "v", "k_cache", "v_cache", "k_scale", "v_scale", "start_ptr"))
+    for m in ((1 << 31) - 1, (1 << 31) - 62, 65534 * 64 + 2):
+        assert _status("L.t5b_cache_quantize(ptr(_c_struct('t5b_cache_quantize_args')(dtype=nat.F16, B=1, H=1, M=%d, D=16, capacity=64, %s)), None)"
+                       % (m, full)) == 2

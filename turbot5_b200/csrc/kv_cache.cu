@@ -347,7 +347,7 @@ extern "C" int t5b_cache_quantize(const t5b_cache_quantize_args* a, void* stream
   if (a->dtype != T5B_F32 && a->dtype != T5B_F16 && a->dtype != T5B_BF16) return T5B_ERR_DTYPE;
   if (a->D != 16 && a->D != 32 && a->D != 64 && a->D != 128) return T5B_ERR_HEAD_DIM;
   if (a->B < 0 || a->H < 0 || a->M < 0 || a->capacity < 0 || a->capacity % T5B_CACHE_BLOCK || a->B > 32767 || a->H > 65535 ||
-      (a->M + T5B_CACHE_BLOCK - 2) / T5B_CACHE_BLOCK + 1 > 65535) return T5B_ERR_SHAPE;
+      a->M > 65534 * T5B_CACHE_BLOCK + 1) return T5B_ERR_SHAPE;
   if (!a->start_ptr && a->start < 0) return T5B_ERR_ARG;
   if (a->B == 0 || a->H == 0 || a->M == 0) return T5B_OK;
   if (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale) return T5B_ERR_ARG;
