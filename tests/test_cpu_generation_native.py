@@ -71,3 +71,11 @@ def test_numbers_of_tokens_near_the_largest_number_are_refused():
     for m in ((1 << 31) - 1, (1 << 31) - 62, 65534 * 64 + 2):
         assert _status("L.t5b_cache_quantize(ptr(_c_struct('t5b_cache_quantize_args')(dtype=nat.F16, B=1, H=1, M=%d, D=16, capacity=64, %s)), None)"
                        % (m, full)) == 2
+
+
+def test_cache_lengths_near_the_largest_number_are_refused():
+    """Rounding up to whole items must not pass 2^31."""
+    full = ", ".join("%s=16" % n for n in ("q", "k", "v", "k_scale", "v_scale", "out"))
+    for n in ((1 << 31) - 1, (1 << 31) - 63):
+        assert _status("L.t5b_decode_quantized_fwd(ptr(_c_struct('t5b_decode_quantized_args')(dtype=nat.F16, B=1, H=1, M=1, N=%d, D=16, %s)), None)"
+                       % (n, full)) == 2

@@ -565,7 +565,8 @@ extern "C" int t5b_decode_quantized_fwd(const t5b_decode_quantized_args* a, void
   if (!a) return T5B_ERR_ARG;
   if (a->dtype != T5B_F16 && a->dtype != T5B_BF16) return T5B_ERR_DTYPE;
   if (a->D != 16 && a->D != 32 && a->D != 64 && a->D != 128) return T5B_ERR_HEAD_DIM;
-  if (a->B < 0 || a->H < 0 || a->M < 0 || a->N < 0 || a->H > 65535 || a->M > (1 << 20)) return T5B_ERR_SHAPE;
+  if (a->B < 0 || a->H < 0 || a->M < 0 || a->N < 0 || a->N > 0x7fffffff - (T5B_CACHE_BLOCK - 1) || a->H > 65535 ||
+      a->M > (1 << 20)) return T5B_ERR_SHAPE;
   if (a->B == 0 || a->H == 0 || a->M == 0) return T5B_OK;
   if (a->q_pos_offset > 0x7fffffff - a->M - 2 * T5B_CACHE_BLOCK) return T5B_ERR_ARG;      // positions are 32-bit numbers
   if (!a->q || !a->out || (a->N > 0 && (!a->k || !a->v || !a->k_scale || !a->v_scale))) return T5B_ERR_ARG;
