@@ -79,3 +79,10 @@ def test_cache_lengths_near_the_largest_number_are_refused():
     for n in ((1 << 31) - 1, (1 << 31) - 63):
         assert _status("L.t5b_decode_quantized_fwd(ptr(_c_struct('t5b_decode_quantized_args')(dtype=nat.F16, B=1, H=1, M=1, N=%d, D=16, %s)), None)"
                        % (n, full)) == 2
+
+
+def test_no_exception_of_an_allocation_leaves_a_c_entry_point():
+    for name in os.listdir(os.path.join(ROOT, "turbot5_b200", "csrc")):
+        if name.endswith((".cu", ".cuh")):
+            text = re.sub(r"//[^\n]*|/\*.*?\*/", "", open(os.path.join(ROOT, "turbot5_b200", "csrc", name)).read(), flags=re.S)
+            assert not re.search(r"\bnew\s+\w|std::(vector|string|map|unordered_map)\b", text), name

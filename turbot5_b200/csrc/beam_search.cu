@@ -39,6 +39,7 @@
 #include <cooperative_groups.h>
 
 #include <atomic>
+#include <new>
 #include <type_traits>
 
 namespace cg = cooperative_groups;
@@ -912,7 +913,8 @@ struct Fit {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     if (const Fit* f = known[dev]) return f;
-    Fit* f = new Fit;                    // kept for the life of the process (a second thread may find the same again)
+    Fit* f = new (std::nothrow) Fit;     // kept for the life of the process (a second thread may find the same again)
+    if (!f) return nullptr;
     if (!resident_clusters((const void*)step_kernel<T, SHORT>, THREADS, 0, f->clusters)) { delete f; return nullptr; }
     known[dev] = f;
     return f;

@@ -38,6 +38,7 @@
 #include <cooperative_groups.h>
 
 #include <atomic>
+#include <new>
 
 namespace cg = cooperative_groups;
 
@@ -486,7 +487,8 @@ struct Fit {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, WARPS * 32, smem) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return nullptr;
-    Fit* f = new Fit;                    // kept for the life of the process (a second thread may find the same again)
+    Fit* f = new (std::nothrow) Fit;     // kept for the life of the process (a second thread may find the same again)
+    if (!f) return nullptr;
     f->resident = per_sm * sms;
     if (!resident_clusters((const void*)kernel, WARPS * 32, smem, f->clusters)) { delete f; return nullptr; }
     known[dev] = f;
