@@ -228,3 +228,38 @@ def test_more_refusals_before_any_step():
         model.beam_search(states, 4, 2, num_return_sequences=0)
     with pytest.raises(ValueError, match="beams"):
         model.generate(torch.zeros((1, 4), dtype=torch.long, device="cuda"), num_beams=0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K,steps", [(6, 70), (12, 9), (16, 9)])
+def test_wide_searches_from_8_bit_caches(K, steps, dtype):
+    """More beams than rows of one pass over the encoder's keys: the choices are the plain search's over the logits, and the
+    logits those of each beam's sentence fed through a cache of its own, which nothing reorders."""
+    B = 2
+    model, states = _model(dtype), _states(B, 150, dtype)
+    search, logits = _recorded(model, states, steps, K, cache_dtype=FP8)
+    state, history = _plain_search(logits, B, K)
+    assert search.history[0].tolist() == history[0] and search.history[1].tolist() == history[1]
+    got, _ = search.sequences(K)
+    assert got.tolist() == plain.sequences(*history, *state, K)[0]
+    tokens, parents = (h.cpu() for h in search.history)
+    last, lines = steps - 1, []
+    for b in range(B):
+        for j in range(K):
+            words, beam = [], j
+            for s in range(last - 1, -1, -1):
+                words.append(int(tokens[s, b, beam]))
+                beam = int(parents[s, b, beam])
+            lines.append([0] + words[::-1])
+    ids = torch.tensor(lines, device="cuda")
+    with torch.no_grad():
+        cache = model.decoder.new_cache(states.repeat_interleave(K, 0), steps, cache_dtype=FP8)
+        for t in range(steps):
+            pos, lens = torch.tensor([t], device="cuda"), torch.full((B * K,), t + 1, dtype=torch.int32, device="cuda")
+            hidden = model.decoder.decode_step_static(ids[:, t:t + 1], cache, pos, lens)
+        want = model.logits(hidden)[:, -1].double().cpu()
+    running = [b * K + j for b in range(B) for j in range(K) if not bool(search.done[b])]
+    assert running
+    # the same arithmetic but for the rows that share a product: 16-bit roundings may fall the other way, and with them
+    # those of the cached keys and values, half a step of e4m3 (2^-4) of some numbers, in two layers
+    assert (logits[last] - want)[running].norm() <= 2 * 2.0 ** -4 * want[running].norm()
