@@ -927,3 +927,28 @@ def test_step_log_sums(B, K, V, std, dtype):
     # on average the roundings cancel.  What remains: an exponential is 5.1e-8 too small (three of them), and log2(e) in
     # float32 1.4e-8 of the distance from the maximum (3 on the weighted average)
     assert off.mean().abs() <= 3 * 5.1e-8 + 3 * 1.4e-8
+
+
+@pytest.mark.parametrize("V", [5000, 140001])
+def test_step_logarithms(V):
+    """Rows of n equal logits: their sum of exponentials is n exactly, and running scores that cancel the logarithm leave
+    its error."""
+    import turbot5_b200 as t5b
+    B, K = 8, 8
+    g = torch.Generator().manual_seed(V)
+    counts = [2, 3, 5, 7, 11, 16, 45, 46, 63, 64, 65, 90, 91, 1448, 1449, 4096] + torch.randint(2, V + 1, (B * K - 16,), generator=g).tolist()
+    logits = torch.full((B * K, V), NONE)
+    for row, n in zip(logits, counts):
+        row[:n] = 1.5
+    logs = torch.tensor([math.log(n) for n in counts], dtype=torch.float64)
+    scores = logs.float()
+    none = torch.zeros((B, K), dtype=torch.int32, device="cuda")
+    _, parents, out, *_ = t5b.beam_search_step(logits.cuda(), scores.view(B, K).cuda(), torch.full((B, K), NONE, device="cuda"), none, none,
+                                               torch.zeros(B, dtype=torch.bool, device="cuda"), torch.zeros(1, dtype=torch.long, device="cuda"),
+                                               eos_token_id=None)
+    rows = (torch.arange(B)[:, None] * K + parents.long().cpu()).flatten()
+    want = scores[rows].double() - logs[rows]
+    # the series' first missing term 2 / 17 * 0.172^17 = 1e-14, a reciprocal of 48 bits, float64 roundings of numbers up to
+    # 12; the result's own, of 2^-21 at most
+    assert ((out.flatten().double().cpu() - want).abs() <= 1e-13 + want.abs() * 2.0 ** -24).all()
+    assert len(set(rows.tolist())) >= B                # (the best row of each sentence at least)
