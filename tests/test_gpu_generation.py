@@ -952,3 +952,36 @@ def test_step_logarithms(V):
     # 12; the result's own, of 2^-21 at most
     assert ((out.flatten().double().cpu() - want).abs() <= 1e-13 + want.abs() * 2.0 ** -24).all()
     assert len(set(rows.tolist())) >= B                # (the best row of each sentence at least)
+
+
+def test_caches_between_and_over_one_another_rows():
+    """Views with gaps: refused where two of them share bytes, wherever that is, and taken where they lie between one
+    another's rows, heads or tokens."""
+    import turbot5_b200 as t5b
+    parents = torch.tensor([[1, 0], [0, 0]], dtype=torch.int32, device="cuda")
+    base = torch.arange(4 * 3 * 128 * 16, device="cuda").view(4, 3, 128, 16) % 251
+    rows = [1, 0, 2, 2]
+    for a, b in ((slice(0, 64), slice(32, 96)), (slice(0, 64), slice(63, 127)), (slice(5, 8), slice(6, 9))):
+        got = base.to(torch.uint8)
+        with pytest.raises(ValueError, match="overlap"):
+            t5b.reorder_beam_cache([got[:, :, a], got[:, :, b]], parents)
+        assert torch.equal(got, base.to(torch.uint8))
+    got = base.to(torch.uint8)
+    with pytest.raises(ValueError, match="overlap"):
+        t5b.reorder_beam_cache([got[:, :, :32], got[:, :, 64:96], got[:, :, 90:122]], parents)
+    with pytest.raises(ValueError, match="overlap"):
+        t5b.reorder_beam_cache([got[:, :2], got[:, 1:]], parents)
+    t5b.reorder_beam_cache([got[:, :, :64], got[:, :, 64:]], parents)
+    assert torch.equal(got, base.to(torch.uint8)[rows])
+    got = base.to(torch.uint8)
+    t5b.reorder_beam_cache([got[:, h:h + 1] for h in (2, 0, 1)], parents)
+    assert torch.equal(got, base.to(torch.uint8)[rows])
+    x = torch.ones((4, 1, 5, 16), device="cuda", dtype=torch.bfloat16)
+    cache, scale = torch.zeros((4, 3, 192, 16), device="cuda").to(FP8), torch.ones((4, 3, 2, 2), device="cuda")
+    with pytest.raises(ValueError, match="own"):
+        t5b.quantize_into_cache(x, x, cache[:, :1, :128], scale[:, :1, 0], cache[:, :1, 64:], scale[:, :1, 1])
+    with pytest.raises(ValueError, match="own"):
+        t5b.quantize_into_cache(x, x, cache[:, :1, :64], scale[:, :1, 0, :1], cache[:, :1, 64:128], scale[:, :1, 0, :1])
+    t5b.quantize_into_cache(x, x * 2, cache[:, :1, :64], scale[:, :1, 0, :1], cache[:, :1, 64:128], scale[:, :1, 1, 1:])
+    back = lambda c, s: (c[:, :, :5].float() * s[..., None]).unique().tolist()
+    assert back(cache[:, :1, :64], scale[:, :1, 0, :1]) == [1.0] and back(cache[:, :1, 64:128], scale[:, :1, 1, 1:]) == [2.0]

@@ -47,6 +47,35 @@ struct Span {
   }
   bool meets(const Span& o) const { return from < o.to && o.from < to; }
 };
+// Whether two tensors of one shape and one set of strides, `delta` bytes apart, share a byte.  Dim by dim from the widest
+// stride: where a dim's stride holds all that is inside it, only two distances of its index can make up for `delta`.
+struct Dim { int64_t stride, size; };
+bool share_bytes(int64_t delta, const Dim* dims, size_t n, int64_t es) {
+  if (n == 0) return std::abs(delta) < es;
+  int64_t q = delta / dims->stride;
+  if (q * dims->stride > delta) --q;
+  for (int64_t c = q; c <= q + 1; ++c)
+    if (std::abs(c) < dims->size && share_bytes(delta - c * dims->stride, dims + 1, n - 1, es)) return true;
+  return false;
+}
+// Equal tensors that share a byte, if there are two.
+bool any_share_bytes(const std::vector<Tensor>& ts) {
+  const Tensor& t0 = ts[0];
+  if (t0.numel() == 0) return false;
+  const int64_t es = t0.element_size();
+  std::vector<Dim> dims;
+  for (int64_t d = 0; d < t0.dim(); ++d)
+    if (t0.size(d) > 1) dims.push_back({t0.stride(d) * es, t0.size(d)});
+  std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
+  const Span whole(t0);
+  std::vector<uintptr_t> at;
+  for (const Tensor& t : ts) at.push_back((uintptr_t)t.data_ptr());
+  std::sort(at.begin(), at.end());
+  for (size_t i = 0; i < at.size(); ++i)
+    for (size_t j = i + 1; j < at.size() && at[j] - at[i] < whole.to - whole.from; ++j)
+      if (share_bytes((int64_t)(at[j] - at[i]), dims.data(), dims.size(), es)) return true;
+  return false;
+}
 // `n` lengths on the device
 Tensor lengths_arg(PyObject* o, int64_t n, at::Device dev, const char* name) {
   const Tensor t = tensor_arg(o);
@@ -246,13 +275,7 @@ Rows rows_of(const std::vector<Tensor>& ts, int64_t dims, int64_t R, at::Device 
     check_on(t, dev, name);
     check_written(t, name, grad);
   }
-  if (t0.numel() == 0) return r;
-  // tensors without gaps overlap where their spans do; others may lie between one another's rows
-  std::vector<uintptr_t> at;
-  for (const Tensor& t : ts) at.push_back((uintptr_t)t.data_ptr());
-  std::sort(at.begin(), at.end());
-  const uintptr_t apart = t0.is_non_overlapping_and_dense() ? (uintptr_t)t0.numel() * es : 1;
-  for (size_t i = 1; i < at.size(); ++i) TORCH_CHECK_VALUE(at[i] - at[i - 1] >= apart, name, ": the same tensor twice, or two that overlap");
+  TORCH_CHECK_VALUE(!any_share_bytes(ts), name, ": the same tensor twice, or two that overlap");
   return r;
 }
 
@@ -346,10 +369,7 @@ PyObject* py_cache_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   check_cache(kc, ks, B, H, D, dev, "k_cache"); check_cache(vc, vs, B, H, D, dev, "v_cache");
   for (const Tensor* t : {&kc, &vc, &ks, &vs}) check_written(*t, "the cache", grad);
   TORCH_CHECK_VALUE(kc.sizes() == vc.sizes() && kc.strides() == vc.strides() && ks.strides() == vs.strides(), "k_cache and v_cache must be alike in shape and strides");
-  const auto apart = [](const Tensor& x, const Tensor& y) {       // (tensors with gaps may lie between one another's rows)
-    return x.numel() == 0 || (x.data_ptr() != y.data_ptr() && !(x.is_non_overlapping_and_dense() && Span(x).meets(Span(y))));
-  };
-  TORCH_CHECK_VALUE(apart(kc, vc) && apart(ks, vs), "keys and values need caches of their own");
+  TORCH_CHECK_VALUE(!any_share_bytes({kc, vc}) && !any_share_bytes({ks, vs}), "keys and values need caches of their own");
   const int64_t cap = kc.size(2);
   t5b_cache_quantize_args g;
   g.start_ptr = nullptr; g.start = 0;
