@@ -985,3 +985,23 @@ def test_caches_between_and_over_one_another_rows():
     t5b.quantize_into_cache(x, x * 2, cache[:, :1, :64], scale[:, :1, 0, :1], cache[:, :1, 64:128], scale[:, :1, 1, 1:])
     back = lambda c, s: (c[:, :, :5].float() * s[..., None]).unique().tolist()
     assert back(cache[:, :1, :64], scale[:, :1, 0, :1]) == [1.0] and back(cache[:, :1, 64:128], scale[:, :1, 1, 1:]) == [2.0]
+
+
+def test_caches_that_overlap_themselves_are_refused():
+    import turbot5_b200 as t5b
+    parents = torch.tensor([[1, 0], [0, 0]], dtype=torch.int32, device="cuda")
+    base = torch.zeros(4 * 3 * 128 * 16, device="cuda", dtype=torch.uint8)
+    x = torch.ones((4, 1, 5, 16), device="cuda", dtype=torch.bfloat16)
+    scale = [torch.ones((4, 1, 2), device="cuda") for _ in range(2)]
+    # rows that begin inside of one another, heads that do, one row for all
+    for sizes, strides in (((4, 1, 128, 16), (1024, 2048, 16, 1)), ((4, 3, 128, 16), (6144, 2032, 16, 1)), ((4, 1, 128, 16), (0, 2048, 16, 1))):
+        windows = base.as_strided(sizes, strides)
+        with pytest.raises(ValueError, match="itself"):
+            t5b.reorder_beam_cache([windows], parents)
+        if sizes[1] == 1:
+            with pytest.raises(ValueError, match="itself"):
+                t5b.quantize_into_cache(x, x, windows.view(FP8), scale[0], torch.zeros((4, 1, 128, 16), device="cuda").to(FP8), scale[1])
+    # any order of dims, steps over rows, and sizes of one with any stride are none of that
+    t5b.reorder_beam_cache([base.view(3, 4, 128, 16).transpose(0, 1)], parents)
+    t5b.reorder_beam_cache([base.view(8, 3, 64, 16)[::2]], parents)
+    t5b.reorder_beam_cache([base.as_strided((4, 1, 128, 16), (2048, 1, 16, 1))], parents)

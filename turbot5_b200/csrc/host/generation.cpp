@@ -1,7 +1,6 @@
 // Beam search and 8-bit caches: argument checks, outputs and launches, and their Python bindings.
 #include "host.h"
 
-#include <ATen/MemoryOverlap.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -28,9 +27,25 @@ void check_plain(const Tensor& t, at::ScalarType dtype, at::IntArrayRef sizes, a
   check_on(t, dev, name);
   TORCH_CHECK_VALUE(t.is_contiguous(), name, " must be contiguous");
 }
-// Tensors that are written in place: they do not overlap themselves, have no part in gradients, and count the change.
+struct Dim { int64_t stride, size; };
+// A tensor's dims with more than one index, widest stride first.
+std::vector<Dim> dims_of(const Tensor& t) {
+  std::vector<Dim> dims;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1) dims.push_back({t.stride(d), t.size(d)});
+  std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
+  return dims;
+}
+// Tensors that are written in place: they do not overlap themselves (every stride reaches past what is inside it), have
+// no part in gradients, and count the change.
 void check_written(const Tensor& t, const char* name, bool grad) {
-  TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, name, " is written and must not overlap itself");
+  int64_t inside = 0;
+  bool apart = true;
+  if (t.numel() > 0 && !t.is_non_overlapping_and_dense()) {
+    const std::vector<Dim> dims = dims_of(t);
+    for (size_t i = dims.size(); i-- > 0; inside += (dims[i].size - 1) * dims[i].stride) apart = apart && dims[i].stride > inside;
+  }
+  TORCH_CHECK_VALUE(apart, name, " is written and must not overlap itself");
   TORCH_CHECK_VALUE(!(grad && t.requires_grad()), name, " is written in place and must not require gradients");
 }
 void count_change(const Tensor& t) {
@@ -49,7 +64,6 @@ struct Span {
 };
 // Whether two tensors of one shape and one set of strides, `delta` bytes apart, share a byte.  Dim by dim from the widest
 // stride: where a dim's stride holds all that is inside it, only two distances of its index can make up for `delta`.
-struct Dim { int64_t stride, size; };
 bool share_bytes(int64_t delta, const Dim* dims, size_t n, int64_t es) {
   if (n == 0) return std::abs(delta) < es;
   int64_t q = delta / dims->stride;
@@ -58,22 +72,19 @@ bool share_bytes(int64_t delta, const Dim* dims, size_t n, int64_t es) {
     if (std::abs(c) < dims->size && share_bytes(delta - c * dims->stride, dims + 1, n - 1, es)) return true;
   return false;
 }
-// Equal tensors that share a byte, if there are two.
-bool any_share_bytes(const std::vector<Tensor>& ts) {
-  const Tensor& t0 = ts[0];
-  if (t0.numel() == 0) return false;
-  const int64_t es = t0.element_size();
+// Of tensors that are alike in shape and strides, with these first bytes: whether two share a byte.
+bool any_share_bytes(const Tensor& like, uintptr_t* at, size_t n) {
+  std::sort(at, at + n);
+  const Span whole(like);
   std::vector<Dim> dims;
-  for (int64_t d = 0; d < t0.dim(); ++d)
-    if (t0.size(d) > 1) dims.push_back({t0.stride(d) * es, t0.size(d)});
-  std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
-  const Span whole(t0);
-  std::vector<uintptr_t> at;
-  for (const Tensor& t : ts) at.push_back((uintptr_t)t.data_ptr());
-  std::sort(at.begin(), at.end());
-  for (size_t i = 0; i < at.size(); ++i)
-    for (size_t j = i + 1; j < at.size() && at[j] - at[i] < whole.to - whole.from; ++j)
-      if (share_bytes((int64_t)(at[j] - at[i]), dims.data(), dims.size(), es)) return true;
+  for (size_t i = 0; i < n; ++i)
+    for (size_t j = i + 1; j < n && at[j] - at[i] < whole.to - whole.from; ++j) {
+      if (dims.empty()) {
+        dims = dims_of(like);
+        for (Dim& d : dims) d.stride *= like.element_size();
+      }
+      if (share_bytes((int64_t)(at[j] - at[i]), dims.data(), dims.size(), like.element_size())) return true;
+    }
   return false;
 }
 // `n` lengths on the device
@@ -275,7 +286,9 @@ Rows rows_of(const std::vector<Tensor>& ts, int64_t dims, int64_t R, at::Device 
     check_on(t, dev, name);
     check_written(t, name, grad);
   }
-  TORCH_CHECK_VALUE(!any_share_bytes(ts), name, ": the same tensor twice, or two that overlap");
+  std::vector<uintptr_t> at;
+  for (const Tensor& t : ts) at.push_back((uintptr_t)t.data_ptr());
+  TORCH_CHECK_VALUE(!any_share_bytes(t0, at.data(), at.size()), name, ": the same tensor twice, or two that overlap");
   return r;
 }
 
@@ -369,7 +382,8 @@ PyObject* py_cache_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   check_cache(kc, ks, B, H, D, dev, "k_cache"); check_cache(vc, vs, B, H, D, dev, "v_cache");
   for (const Tensor* t : {&kc, &vc, &ks, &vs}) check_written(*t, "the cache", grad);
   TORCH_CHECK_VALUE(kc.sizes() == vc.sizes() && kc.strides() == vc.strides() && ks.strides() == vs.strides(), "k_cache and v_cache must be alike in shape and strides");
-  TORCH_CHECK_VALUE(!any_share_bytes({kc, vc}) && !any_share_bytes({ks, vs}), "keys and values need caches of their own");
+  uintptr_t caches[2] = {(uintptr_t)kc.data_ptr(), (uintptr_t)vc.data_ptr()}, scales[2] = {(uintptr_t)ks.data_ptr(), (uintptr_t)vs.data_ptr()};
+  TORCH_CHECK_VALUE(!any_share_bytes(kc, caches, 2) && !any_share_bytes(ks, scales, 2), "keys and values need caches of their own");
   const int64_t cap = kc.size(2);
   t5b_cache_quantize_args g;
   g.start_ptr = nullptr; g.start = 0;
