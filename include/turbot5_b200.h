@@ -450,8 +450,9 @@ T5B_API int t5b_beam_search_sequences(const t5b_beam_sequences_args* args, void*
  * In place, for every tensor: row[b * num_beams + j] = row[b * num_beams + parents[b, j]] (all read before any is
  * written), for the tokens in use.  caches: device pointers to (outer, B * num_beams, H, capacity, token) with byte
  * strides for the first three dims and token_bytes contiguous bytes per token; scales: float32 (outer, B * num_beams, H,
- * ceil(capacity / 64)), byte strides, last dim contiguous; not without caches (T5B_ERR_ARG).  seqlens: optional int32 (B * num_beams), tokens in use (the
- * longest beam of a sentence counts); NULL: the capacity.  A parent outside the beams leaves its row as it is. */
+ * ceil(capacity / 64)), byte strides, last dim contiguous; not without caches (T5B_ERR_ARG).  seqlens: optional int32
+ * (B * num_beams), tokens in use (the longest beam of a sentence counts); NULL: the capacity.  A parent outside the beams
+ * leaves its row as it is. */
 #define T5B_CACHE_BLOCK 64
 #define T5B_REORDER_MAX_TENSORS 64
 typedef struct {

@@ -139,9 +139,9 @@ def flash_decoding_quantized_with_fusing_bias(q, k, k_scale, v, v_scale, bias, c
     `quantize_into_cache` leaves them.
 
     Half of the bytes of a 16-bit cache are read; up to eight query rows (the beams of a sentence against its encoder's
-    keys) cost one pass over them.  Only the first `kv_len` (`seqlens_k[b]`) keys are read; a row that sees none gives
-    zeros.  A key that is visible to some rows of a causal call only must hold finite numbers: 0 x NaN is NaN.  No
-    workspace and no state: calls on any streams are independent.  No gradients are recorded."""
+    keys) cost one pass over them, and every eight rows more another one.  Only the first `kv_len` (`seqlens_k[b]`) keys
+    are read; a row that sees none gives zeros.  A key that is visible to some rows of a causal call only must hold finite
+    numbers: 0 x NaN is NaN.  No workspace and no state: calls on any streams are independent.  No gradients are recorded."""
     return _host.decode_quantized(q, k, k_scale, v, v_scale, bias, causal, sm_scale, NUM_BUCKETS, MAX_DISTANCE, kv_len,
                                   seqlens_k, q_pos_offset)
 

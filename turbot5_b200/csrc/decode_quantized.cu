@@ -519,7 +519,9 @@ static int launch(const Params& p, const BucketSpec& spec, int C, cudaStream_t s
 //   * short caches of many heads: two warps (768 x 512: 12.8, with four 14.3), and more heads than blocks of four warps are
 //     resident, up to half as many more (512 x 4096 of 128 columns: 96.8, with four 115.7);
 //   * else four warps (1536 x 2048: 66.9, with two 78.8), two blocks per head for long caches of 400 to 1200 heads, where
-//     one block per head leaves the last round of blocks half empty (1024 x 8192: 165.5, with one 170.2).
+//     one block per head leaves the last round of blocks half empty (x 8192, two blocks and one: 448 heads 84 and 89, 640
+//     115 and 136, 768 129 and 146, 1024 173 and 181, 1152 197 and 190; of 128 columns 448 heads 176 and 198, 640 217 and
+//     256, 1024 352 and 357; x 4096 neither is ahead: 448 heads 47.5 and 47.2, 640 64.0 and 65.1, 1024 90.9 and 91.0).
 template <typename T, int D, int TILES>
 static int launch_split(const Params& p, const BucketSpec& spec, cudaStream_t stream) {
   const int64_t heads = (int64_t)p.B * p.H * p.row_groups, items = (p.N + Ring<D>::ITEM - 1) / Ring<D>::ITEM;

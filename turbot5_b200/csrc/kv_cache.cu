@@ -209,7 +209,7 @@ fill_kernel(const __grid_constant__ FillParams p) {
 // nothing costs as much as one that moves 16 KB: heads share a few hundred blocks, each of which takes piece after piece,
 // and short heads get blocks of 64 threads.  16 beams of 104 of 470 tokens (92 MB): 24 us, 77 with a block per piece; 3
 // beams of 37 of 229 tokens in 24 layers (65 MB): 19 and 40.
-constexpr int REORDER_THREADS = 2 * 148 * 256;             // beyond these a block takes several pieces of a head
+constexpr int REORDER_THREADS = 2 * 148 * 256;             // (148 multiprocessors) beyond these a block takes several pieces
 
 constexpr int in_flight(int beams) { return beams == 16 ? 1 : 2; }
 
