@@ -1005,3 +1005,31 @@ def test_caches_that_overlap_themselves_are_refused():
     t5b.reorder_beam_cache([base.view(3, 4, 128, 16).transpose(0, 1)], parents)
     t5b.reorder_beam_cache([base.view(8, 3, 64, 16)[::2]], parents)
     t5b.reorder_beam_cache([base.as_strided((4, 1, 128, 16), (2048, 1, 16, 1))], parents)
+
+
+@pytest.mark.parametrize("B,K,V", [(100, 16, 128256), (300, 4, 32128), (64, 10, 50001), (148, 8, 20000), (700, 2, 9001)])
+def test_step_of_large_batches(B, K, V):
+    """Batches whose sentences have few blocks each, wide vocabularies: the best continuations against float64 sorting."""
+    import turbot5_b200 as t5b
+    g = torch.Generator(device="cuda").manual_seed(V)
+    logits = torch.randn((B * K, V), generator=g, device="cuda") * 2.5
+    scores = -torch.rand((B, K), generator=g, device="cuda") * 4
+    none = torch.zeros((B, K), dtype=torch.int32, device="cuda")
+    tokens, parents, out, *_ = t5b.beam_search_step(logits, scores, torch.full((B, K), NONE, device="cuda"), none, none,
+                                                    torch.zeros(B, dtype=torch.bool, device="cuda"), torch.zeros(1, dtype=torch.long, device="cuda"),
+                                                    eos_token_id=None)
+    compared = 0
+    for b in range(B):
+        every = scores[b].double()[:, None] + logits[b * K:(b + 1) * K].double().log_softmax(-1)
+        best = every.flatten().topk(K + 1)
+        values = best.values.tolist()
+        # what log-sums are off by (1e-6 covers the bound, both ways) may turn the last place around, in a few sentences
+        if values[K - 1] - values[K] < 2e-6:
+            continue
+        compared += 1
+        assert sorted(best.indices[:K].tolist()) == sorted((parents[b].long() * V + tokens[b]).tolist()), b
+        got = out[b].double().sort(descending=True)[0]
+        assert ((got - best.values[:K]).abs() <= best.values[:K].abs() * 2.0 ** -24 + 1e-6).all()
+        for j in range(K):                             # a beam that goes on keeps its place once
+            assert int(parents[b, j]) == j or j not in parents[b].tolist()
+    assert compared >= B * 0.99 - 1
