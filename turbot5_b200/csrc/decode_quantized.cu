@@ -25,8 +25,8 @@
 // A warp works on items of 32 or 64 keys of one block of 64 (so an item has one scale), with its own running maximum and
 // sum and its own ring of stages in shared memory that asynchronous copies fill ahead (registers alone held too little in
 // flight: 206 us for 1.07 GB, 166 with the ring, the floor at the measured copy rate 164).  That is at 1965 MHz, in bursts
-// of some milliseconds.  A second of it draws the 1000 W that the GPU may take, the clock falls to 1450 MHz and issue slots
-// decide: 188 us, 193 as calls one behind the other.  Warps merge in shared memory, the blocks
+// of some milliseconds.  A second of it draws the 1000 W that the GPU may take, and with the clock at 1450 MHz it takes 188
+// us, 193 as calls one behind the other (half of the issue slots are taken).  Warps merge in shared memory, the blocks
 // of a (batch, head) that share a long cache form a cluster and merge through distributed shared memory: no workspace,
 // no counters, no second launch.  The bias is looked up for items within the largest distance of a query only, from a
 // table of the item's distances that the warp makes for itself.
